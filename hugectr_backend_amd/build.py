@@ -30,6 +30,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 CXXFLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter", "-pthread",
             f"-I{ROOT / 'include'}", f"-I{CSRC}", *os.environ.get("HPS_AMD_EXTRA_FLAGS", "").split()]
+# device code only: some packed fp32 instructions that hipcc makes of plain float code have given wrong results on this chip
+HIPFLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 ENGINE_SRCS = [
     "common/json.cpp",
@@ -47,12 +49,16 @@ ENGINE_SRCS = [
     "cache/copy_engines.cpp",
     "cache/segcopy_kernels.hip",
     "cache/probe_kernels.hip",
+    "cache/qrows_kernels.hip",
     "cache/multi_gpu_probe.cpp",
     "cache/engine.cpp",
     "cache/parameter_server.cpp",
     "dense/dense_kernels.hip",
     "dense/fused_kernels.hip",
     "dense/dense.cpp",
+    "dense/linear_kernels.hip",
+    "dense/group_rows.hip",
+    "dense/linear.cpp",
 ]
 CAPI_SRCS = ["c_api.cpp"]
 TRITON_SRCS = [
@@ -74,6 +80,10 @@ def _run(cmd):
     return r
 
 
+def _flags(src: Path) -> list:
+    return HIPFLAGS if src.suffix == ".hip" else []
+
+
 def _deps_stamp(src: Path) -> str:
     """Hash of the source and every header under csrc/ + include/ (coarse but safe)."""
     h = hashlib.sha1()
@@ -81,7 +91,7 @@ def _deps_stamp(src: Path) -> str:
     for d in (CSRC, ROOT / "include"):
         for p in sorted(d.rglob("*.h")):
             h.update(p.read_bytes())
-    h.update(" ".join(CXXFLAGS).encode())
+    h.update(" ".join(CXXFLAGS + _flags(src)).encode())
     return h.hexdigest()
 
 
@@ -93,7 +103,7 @@ def _compile(rel: str, force: bool) -> Path:
     if not force and obj.exists() and stamp.exists() and stamp.read_text() == want:
         return obj
     obj.parent.mkdir(parents=True, exist_ok=True)
-    cmd = [HIPCC, f"--offload-arch={ARCH}", *CXXFLAGS, "-c", str(src), "-o", str(obj)]
+    cmd = [HIPCC, f"--offload-arch={ARCH}", *CXXFLAGS, *_flags(src), "-c", str(src), "-o", str(obj)]
     _run(cmd)
     stamp.write_text(want)
     return obj

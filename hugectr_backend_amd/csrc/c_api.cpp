@@ -17,8 +17,11 @@
 #include "cache/shard_kernels.h"
 #include "cache/shard_entry.h"
 #include "cache/multi_gpu_probe.h"
+#include "cache/qrows.h"
 #include "cache/shard_session.h"
+#include "common/device_guard.h"
 #include "dense/dense.h"
+#include "dense/linear.h"
 
 using namespace hps;
 
@@ -29,6 +32,7 @@ struct hps_server { std::shared_ptr<HierParameterServer> ps; std::vector<std::st
 struct hps_cache { std::shared_ptr<HierParameterServer> ps; std::string model; int device; std::shared_ptr<EmbeddingCache> cache; };
 struct hps_session { std::shared_ptr<HierParameterServer> ps; std::shared_ptr<LookupSession> s; };   // shared: a sharded session built on it keeps it alive
 struct hps_dense { std::unique_ptr<DenseInteraction> d; };
+struct hps_linear { std::unique_ptr<LinearLayers> l; };
 struct hps_shard_group { std::shared_ptr<LocalShardGroup> g; };
 struct hps_shard_entry { std::shared_ptr<HierParameterServer> ps; std::unique_ptr<ShardedEntrySession> s; };   // (s goes first)
 struct hps_shard_session { std::shared_ptr<HierParameterServer> ps; std::unique_ptr<ShardedSession> s; };   // (s goes first)
@@ -805,6 +809,141 @@ int hps_dense_forward(hps_dense_t* dense, const float* d_dense, const float* d_e
   return Guard([&]() -> Status {
     if (!dense) return Error(Code::kInvalidArg, "null argument");
     return dense->d->Forward(d_dense, d_embeddings, batch, d_out_f16, (hipStream_t)stream);
+  });
+}
+
+uint32_t hps_qrows_row_bytes(uint32_t dim, uint32_t bits) { return QRowsRowBytes(dim, bits); }
+
+uint32_t hps_qrows_groups(uint32_t dim, uint32_t group) { return group == 0 || group >= dim ? 1u : (dim + group - 1) / group; }
+
+namespace {
+Status QRowsStore(const hps_qrows_t* store, bool write, QRowsDesc* d) {
+  if (!store) return Error(Code::kInvalidArg, "null argument");
+  if (store->dim == 0 || store->dim > kQRowsMaxDim) return Error(Code::kInvalidArg, "quantised rows: 1..", kQRowsMaxDim, " values per row supported, got ", store->dim);
+  if (store->bits != 8 && store->bits != 4) return Error(Code::kInvalidArg, "quantised rows: 8 or 4 bits per value, got ", store->bits);
+  const uint32_t g = store->group;
+  if (g != 0 && g != 16 && g != 32 && g != 64 && g != 128 && g != 256)
+    return Error(Code::kInvalidArg, "quantised rows: a scale per row (0) or per 16, 32, 64, 128 or 256 values, got ", g);
+  if (store->num_rows && (!store->codes || !store->scales || (write && !store->owner))) return Error(Code::kInvalidArg, "quantised rows: null store pointer");
+  if ((uintptr_t)store->codes % 4 || (uintptr_t)store->scales % 4 || (uintptr_t)store->owner % 4)
+    return Error(Code::kInvalidArg, "quantised rows: codes, scales and owner are 4-byte aligned");
+  d->codes = (uint8_t*)store->codes;
+  d->scales = store->scales;
+  d->owner = store->owner;
+  d->num_rows = store->num_rows;
+  d->dim = store->dim;
+  d->bits = store->bits;
+  d->groups = hps_qrows_groups(store->dim, g);
+  d->group = g;
+  d->row_bytes = QRowsRowBytes(store->dim, store->bits);
+  return Status::Ok();
+}
+Status ElemTypeOf(int type, ElemType* t) {
+  if (type < HPS_TYPE_FP32 || type > HPS_TYPE_BF16) return Error(Code::kInvalidArg, "unknown element type ", type);
+  *t = (ElemType)type;
+  return Status::Ok();
+}
+}  // namespace
+
+int hps_qrows_write_device(int device, const hps_qrows_t* store, const void* d_rows, int type, uint64_t row_stride, const int64_t* d_slots,
+                           uint64_t n, void* d_held, uint64_t held_stride, void* stream) {
+  return Guard([&]() -> Status {
+    QRowsDesc d;
+    ElemType t;
+    HPS_RETURN_IF_ERROR(QRowsStore(store, true, &d));
+    HPS_RETURN_IF_ERROR(ElemTypeOf(type, &t));
+    if (n >= (1ull << 31)) return Error(Code::kUnsupported, "quantised rows: more than 2^31 rows per call");
+    if (n == 0) return Status::Ok();
+    if (!d_rows || !d_slots) return Error(Code::kInvalidArg, "null argument");
+    if (row_stride < d.dim || (d_held && held_stride < d.dim)) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
+    if (d_held && !(d_held == d_rows && held_stride == row_stride)) {
+      const uintptr_t r = (uintptr_t)d_rows, h = (uintptr_t)d_held;
+      const uint64_t rb = ((n - 1) * row_stride + d.dim) * ElemBytes(t), hb = ((n - 1) * held_stride + d.dim) * ElemBytes(t);
+      if (r < h + hb && h < r + rb) return Error(Code::kInvalidArg, "quantised rows: held overlaps the rows without being the same rows");
+    }
+    DeviceGuard guard;
+    HPS_RETURN_IF_ERROR(guard.Enter(device));
+    const hipError_t e = LaunchQRowsWrite(d, d_rows, t, row_stride, d_slots, n, d_held, held_stride, (hipStream_t)stream);
+    if (e != hipSuccess) return Error(Code::kInternal, "quantised rows write launch failed: ", hipGetErrorString(e));
+    return Status::Ok();
+  });
+}
+
+int hps_qrows_read_device(int device, const hps_qrows_t* store, const int64_t* d_slots, uint64_t n, float default_value, void* d_out, int type,
+                          uint64_t out_stride, void* stream) {
+  return Guard([&]() -> Status {
+    QRowsDesc d;
+    ElemType t;
+    HPS_RETURN_IF_ERROR(QRowsStore(store, false, &d));
+    HPS_RETURN_IF_ERROR(ElemTypeOf(type, &t));
+    if (n >= (1ull << 31)) return Error(Code::kUnsupported, "quantised rows: more than 2^31 rows per call");
+    if (n == 0) return Status::Ok();
+    if (!d_slots || !d_out) return Error(Code::kInvalidArg, "null argument");
+    if (out_stride < d.dim) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
+    DeviceGuard guard;
+    HPS_RETURN_IF_ERROR(guard.Enter(device));
+    const hipError_t e = LaunchQRowsRead(d, d_slots, n, default_value, d_out, t, out_stride, (hipStream_t)stream);
+    if (e != hipSuccess) return Error(Code::kInternal, "quantised rows read launch failed: ", hipGetErrorString(e));
+    return Status::Ok();
+  });
+}
+
+int hps_linear_create(int device, uint32_t num_experts, uint32_t in_dim, uint32_t out_dim, int type, int activation, const void* weights,
+                      int weights_type, const float* bias, int on_device, void* stream, hps_linear_t** out) {
+  return Guard([&]() -> Status {
+    if (!out) return Error(Code::kInvalidArg, "null argument");
+    *out = nullptr;
+    ElemType t, w;
+    HPS_RETURN_IF_ERROR(ElemTypeOf(type, &t));
+    HPS_RETURN_IF_ERROR(ElemTypeOf(weights_type, &w));
+    LinearLayers* l = nullptr;
+    HPS_RETURN_IF_ERROR(LinearLayers::Create(device, num_experts, in_dim, out_dim, t, (Activation)activation, weights, w, bias, on_device != 0,
+                                             (hipStream_t)stream, &l));
+    *out = new hps_linear{std::unique_ptr<LinearLayers>(l)};
+    return Status::Ok();
+  });
+}
+
+void hps_linear_destroy(hps_linear_t* layer) { delete layer; }
+
+int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void* stream) {
+  return Guard([&]() -> Status {
+    if (!layer || !args) return Error(Code::kInvalidArg, "null argument");
+    ElemType t;
+    HPS_RETURN_IF_ERROR(ElemTypeOf(args->out_type, &t));
+    LinearArgs a;
+    a.x = args->x;
+    a.x_stride = args->x_stride;
+    a.x_rows = args->x_rows;
+    a.out = args->out;
+    a.out_stride = args->out_stride;
+    a.out_rows = args->out_rows;
+    a.mul = args->mul;
+    a.mul_stride = args->mul_stride;
+    a.residual = args->residual;
+    a.residual_stride = args->residual_stride;
+    a.rows = args->rows;
+    a.offsets = args->offsets;
+    a.rows_in = args->rows_in;
+    a.rows_out = args->rows_out;
+    a.zero_rest = args->zero_rest;
+    return layer->l->Forward(a, t, (hipStream_t)stream);
+  });
+}
+
+uint64_t hps_group_rows_workspace_bytes(uint64_t n, uint32_t num_experts) { return GroupRowsWorkspaceBytes(n, num_experts); }
+
+int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t num_experts, int32_t* d_offsets, int32_t* d_order,
+                          void* d_workspace, void* stream) {
+  return Guard([&]() -> Status {
+    if (num_experts == 0 || num_experts > kMaxExperts) return Error(Code::kInvalidArg, "grouping: 1..", kMaxExperts, " experts supported, got ", num_experts);
+    if (n >= (1ull << 31)) return Error(Code::kUnsupported, "grouping: more than 2^31 rows per call");
+    if (!d_offsets || (n && (!d_ids || !d_order)) || (GroupRowsWorkspaceBytes(n, num_experts) && !d_workspace)) return Error(Code::kInvalidArg, "null argument");
+    DeviceGuard guard;
+    HPS_RETURN_IF_ERROR(guard.Enter(device));
+    const hipError_t e = LaunchGroupRows(d_ids, n, num_experts, d_offsets, d_order, d_workspace, (hipStream_t)stream);
+    if (e != hipSuccess) return Error(Code::kInternal, "grouping launch failed: ", hipGetErrorString(e));
+    return Status::Ok();
   });
 }
 

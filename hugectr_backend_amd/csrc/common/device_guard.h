@@ -1,0 +1,36 @@
+// The calling thread's device for the length of a C entry: the entry's own device inside, the caller's again behind it.
+#pragma once
+#include <hip/hip_runtime_api.h>
+
+#include "status.h"
+
+namespace hps {
+
+class DeviceGuard {
+ public:
+  DeviceGuard() = default;
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+  ~DeviceGuard() {
+    if (restore_ >= 0) (void)hipSetDevice(restore_);
+  }
+  Status Enter(int device) {
+    int ndev = 0;
+    if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0)
+      return Error(Code::kUnavailable, "this call needs a HIP device and none is visible; there is no CPU fallback");
+    if (device < 0 || device >= ndev) return Error(Code::kInvalidArg, "device ", device, " is not visible (", ndev, " HIP devices)");
+    int now = 0;
+    hipError_t e = hipGetDevice(&now);
+    if (e == hipSuccess && now != device) {
+      e = hipSetDevice(device);
+      if (e == hipSuccess) restore_ = now;
+    }
+    if (e != hipSuccess) return Error(Code::kInternal, "selecting device ", device, " failed: ", hipGetErrorString(e));
+    return Status::Ok();
+  }
+
+ private:
+  int restore_ = -1;
+};
+
+}  // namespace hps

@@ -1,6 +1,7 @@
 """Host-side handle of the dense step of BASELINE config 5 (DLRM bottom MLP + dot interaction) — a thin ctypes
-wrapper over the hps_dense_* entry points of libhps_amd.so (include/hps_amd.h).  The arithmetic is the HIP/MFMA
-code in csrc/dense/; torch is used for device buffers only.
+wrapper over the hps_dense_* entry points of libhps_amd.so (include/hps_amd.h) — and of the layers that come behind it:
+LinearLayer, ExpertLayers (hps_linear_*) and group_rows (hps_group_rows_*).  The arithmetic is the HIP/MFMA code in
+csrc/dense/; torch is used for device buffers only.
 """
 from __future__ import annotations
 
@@ -9,6 +10,9 @@ import ctypes as C
 import numpy as np
 
 from . import hps
+from .quantized_rows import _invalid, elem_type, row_stride
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
 
 class DenseInteraction:
@@ -78,3 +82,138 @@ class DenseInteraction:
             self.close()
         except Exception:  # noqa: BLE001
             pass
+
+
+class ExpertLayers:
+    """y = act(x W_e + b_e) * mul + residual for every expert e over its own run of rows, on the matrix cores: operands of `dtype`
+    (fp16 or bf16), sums and everything behind them in fp32, one rounding at the end.
+
+    weights: [num_experts, in_dim, out_dim] (x @ W convention), biases: None or [num_experts, out_dim]; numpy arrays or torch tensors,
+    laid out for the kernels once, here.  activation: none, relu, gelu (with the error function), silu, sigmoid."""
+
+    def __init__(self, weights, biases=None, activation: str = "none", dtype="fp16", device: int = 0):
+        import torch
+        if hps.device_count() <= 0:
+            raise hps.HpsError(hps.ERR_UNAVAILABLE, "dense layers need a HIP device and none is visible; there is no CPU fallback")
+        dtype = {"fp16": torch.float16, "bf16": torch.bfloat16}.get(dtype, dtype)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise _invalid(f"dense layers take fp16 or bf16 operands, got {dtype}")
+        if activation not in ACTIVATIONS:
+            raise _invalid(f"activation: one of {', '.join(ACTIVATIONS)} expected, got {activation!r}")
+        dev = torch.device("cuda", int(device))
+        w = torch.as_tensor(weights)
+        if w.dim() != 3:
+            raise _invalid(f"weights: [num_experts, in_dim, out_dim] expected, got shape {tuple(w.shape)}")
+        if w.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            w = w.float()
+        w = w.to(dev).contiguous()
+        b = None
+        if biases is not None:
+            b = torch.as_tensor(biases).to(device=dev, dtype=torch.float32).contiguous()
+            if tuple(b.shape) != (w.shape[0], w.shape[2]):
+                raise _invalid(f"biases: [{w.shape[0]}, {w.shape[2]}] expected, got {tuple(b.shape)}")
+        self.num_experts, self.in_dim, self.out_dim = (int(v) for v in w.shape)
+        self.dtype, self.activation, self.device = dtype, activation, int(device)
+        h = C.c_void_p()
+        hps._check(hps.LIB.hps_linear_create(self.device, self.num_experts, self.in_dim, self.out_dim, elem_type(dtype),
+                                             ACTIVATIONS[activation], w.data_ptr(), elem_type(w.dtype), b.data_ptr() if b is not None else None,
+                                             1, torch.cuda.current_stream(dev).cuda_stream, C.byref(h)))
+        self._h = h
+
+    def _index(self, t, n, name):
+        import torch
+        if t is None:
+            return None
+        if not t.is_cuda or t.device.index != self.device or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (
+                n > 1 and t.stride(0) != 1):
+            raise _invalid(f"{name}: a contiguous vector of {n} int32 on cuda:{self.device} expected, got {t.dtype} {tuple(t.shape)} on "
+                           f"{t.device}")
+        return t.data_ptr()
+
+    def forward(self, x, offsets, rows_in=None, rows_out=None, mul=None, residual=None, out=None, out_dtype=None):
+        """x: CUDA `dtype` [x_rows, in_dim] (rows may be apart).  offsets: CUDA int32 [num_experts + 1]; expert e has the positions
+        [offsets[e], offsets[e+1]) (clamped to the positions there are, read as their running maximum).  rows_in / rows_out: None or
+        CUDA int32, one entry per position: the row of x it reads (outside x: zeros) and the row of out, mul and residual it has
+        (outside out: not written; a row named twice holds, element by element, the result of either).
+        Without them position p is row p.  group_rows() makes offsets and such an index from expert numbers.
+        out: [rows, out_dim] of `dtype` or fp32; rows of no run stay as they were.  Without `out` a new tensor of `out_dtype` is
+        returned, one row per position, and rows of no run are zero (rows_out then names every row once).
+        mul, residual: None or `dtype`, rows like out's; either may be `out` itself.
+        Runs on torch's current stream; may be captured; calls may overlap."""
+        p = rows_in if rows_in is not None else rows_out
+        rows = x.shape[0] if p is None else p.shape[0]
+        return self._run(x, rows, self._index(offsets, self.num_experts + 1, "offsets"), self._index(rows_in, rows, "rows_in"),
+                         self._index(rows_out, rows, "rows_out"), mul, residual, out, out_dtype)
+
+    def _run(self, x, rows, offsets, rows_in, rows_out, mul, residual, out, out_dtype):
+        import torch
+        if x.dtype != self.dtype:
+            raise _invalid(f"x: {self.dtype} expected, got {x.dtype}")
+        a = hps.LinearArgs()
+        a.x_stride, a.x, a.x_rows = row_stride(x, self.in_dim, "x", self.device), x.data_ptr(), x.shape[0]
+        if out is None:
+            out = torch.empty((rows, self.out_dim), dtype=out_dtype or self.dtype, device=x.device)
+            a.zero_rest = 1
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
+        a.out_stride, a.out, a.out_rows = row_stride(out, self.out_dim, "out", self.device), out.data_ptr(), out.shape[0]
+        a.out_type = elem_type(out.dtype)
+        if mul is not None:
+            a.mul, a.mul_stride = self._beside(mul, out, "mul")
+        if residual is not None:
+            a.residual, a.residual_stride = self._beside(residual, out, "residual")
+        a.rows, a.offsets, a.rows_in, a.rows_out = rows, offsets, rows_in, rows_out
+        hps._check(hps.LIB.hps_linear_forward(self._h, C.addressof(a), torch.cuda.current_stream(self.device).cuda_stream))
+        return out
+
+    def _beside(self, t, out, name):
+        stride = row_stride(t, self.out_dim, name, self.device)
+        if t.dtype != self.dtype or t.shape[0] != out.shape[0]:
+            raise _invalid(f"{name}: {out.shape[0]} rows of {self.dtype} expected, got {t.shape[0]} of {t.dtype}")
+        return t.data_ptr(), stride
+
+    def close(self):
+        if getattr(self, "_h", None):
+            hps.LIB.hps_linear_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001
+            pass
+
+
+class LinearLayer(ExpertLayers):
+    """y = act(x W + b) * mul + residual: one layer over all rows.  weight: [in_dim, out_dim], bias: None or [out_dim]; the rest as in
+    ExpertLayers."""
+
+    def __init__(self, weight, bias=None, activation: str = "none", dtype="fp16", device: int = 0):
+        super().__init__(weight[None], None if bias is None else bias[None], activation, dtype, device)
+
+    def forward(self, x, mul=None, residual=None, out=None, out_dtype=None):
+        """x: CUDA `dtype` [rows, in_dim]; out, mul, residual: [rows, out_dim] as in ExpertLayers.forward.  Runs on torch's current
+        stream; may be captured; calls may overlap."""
+        if out is not None and out.shape[0] != x.shape[0]:
+            raise _invalid(f"out: {x.shape[0]} rows expected, got {out.shape[0]}")
+        return self._run(x, x.shape[0], None, None, None, mul, residual, out, out_dtype)
+
+
+def group_rows(ids, num_experts: int):
+    """(offsets, order) of a stable sort of the positions by expert number: ids CUDA int32 [n]; offsets int32 [num_experts + 1],
+    order int32 [n]: expert e has the positions order[offsets[e] : offsets[e+1]] in ascending order; positions whose id is outside
+    [0, num_experts) come behind the last run.  num_experts <= 1024.  Runs on torch's current stream; may be captured."""
+    import torch
+    if not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or (ids.shape[0] > 1 and ids.stride(0) != 1):
+        raise _invalid(f"ids: a contiguous CUDA vector of int32 expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+    if not 1 <= num_experts <= 1024:
+        raise _invalid(f"grouping: 1..1024 experts supported, got {num_experts}")
+    n = ids.shape[0]
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=ids.device)
+    order = torch.empty(n, dtype=torch.int32, device=ids.device)
+    nbytes = int(hps.LIB.hps_group_rows_workspace_bytes(n, num_experts))
+    work = torch.empty(nbytes, dtype=torch.uint8, device=ids.device) if nbytes else None
+    hps._check(hps.LIB.hps_group_rows_device(ids.device.index, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
+                                             work.data_ptr() if work is not None else None,
+                                             torch.cuda.current_stream(ids.device).cuda_stream))
+    return offsets, order

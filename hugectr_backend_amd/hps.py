@@ -84,6 +84,18 @@ class RefreshStats(C.Structure):
                 ("keys_changed", C.c_uint64), ("rows_refreshed", C.c_uint64), ("row_bytes", C.c_uint64), ("seconds", C.c_double)]
 
 
+class QRowsStore(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("owner", C.c_void_p), ("num_rows", C.c_uint64), ("dim", C.c_uint32),
+                ("bits", C.c_uint32), ("group", C.c_uint32)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_uint64), ("x_rows", C.c_uint64), ("out", C.c_void_p), ("out_stride", C.c_uint64),
+                ("out_rows", C.c_uint64), ("out_type", C.c_int32), ("zero_rest", C.c_int32), ("mul", C.c_void_p),
+                ("mul_stride", C.c_uint64), ("residual", C.c_void_p), ("residual_stride", C.c_uint64), ("rows", C.c_uint64),
+                ("offsets", C.c_void_p), ("rows_in", C.c_void_p), ("rows_out", C.c_void_p)]
+
+
 class ShardEntryStats(C.Structure):
     _fields_ = [("keys", C.c_uint64), ("unique_keys", C.c_uint64), ("misses", C.c_uint64), ("unique_misses", C.c_uint64),
                 ("bucket_ms", C.c_float), ("lookup_ms", C.c_float), ("expand_ms", C.c_float), ("key_stage_ms", C.c_float),
@@ -181,6 +193,15 @@ def _load() -> C.CDLL:
         "hps_dense_out_stride": (u32, [P]),
         "hps_dense_forward": (C.c_int, [P, P, P, u64, P, P]),
         "hps_session_lookup_interact_device": (C.c_int, [P, P, P, u64, P, P]),
+        "hps_qrows_row_bytes": (u32, [u32, u32]),
+        "hps_qrows_groups": (u32, [u32, u32]),
+        "hps_qrows_write_device": (C.c_int, [C.c_int, P, P, C.c_int, u64, P, u64, P, u64, P]),
+        "hps_qrows_read_device": (C.c_int, [C.c_int, P, P, u64, C.c_float, P, C.c_int, u64, P]),
+        "hps_linear_create": (C.c_int, [C.c_int, u32, u32, u32, C.c_int, C.c_int, P, C.c_int, P, C.c_int, P, C.POINTER(P)]),
+        "hps_linear_destroy": (None, [P]),
+        "hps_linear_forward": (C.c_int, [P, P, P]),
+        "hps_group_rows_workspace_bytes": (u64, [u64, u32]),
+        "hps_group_rows_device": (C.c_int, [C.c_int, P, u64, u32, P, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)  # AttributeError here = symbol missing from the library
@@ -210,6 +231,8 @@ EXPORTED_SYMBOLS = [
     "hps_server_get_shard_cache", "hps_shard_entry_create", "hps_shard_entry_destroy", "hps_shard_entry_lookup",
     "hps_shard_entry_lookup_device", "hps_shard_entry_last_stats", "hps_shard_entry_set_option", "hps_shard_entry_shard_capacity",
     "hps_shard_plan_passes", "hps_multi_gpu_selftest",
+    "hps_qrows_row_bytes", "hps_qrows_groups", "hps_qrows_write_device", "hps_qrows_read_device",
+    "hps_linear_create", "hps_linear_destroy", "hps_linear_forward", "hps_group_rows_workspace_bytes", "hps_group_rows_device",
 ]
 
 

@@ -444,6 +444,83 @@ int hps_dense_forward(hps_dense_t* dense, const float* d_dense, const float* d_e
 int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dense, const int64_t* d_keys_flat, uint64_t batch,
                                        const float* d_dense, void* d_out_f16);
 
+/* ---- element types of the entries below */
+#define HPS_TYPE_FP32 0
+#define HPS_TYPE_FP16 1
+#define HPS_TYPE_BF16 2
+
+/* ---- rows held in 8 or 4 bits, addressed by slot (csrc/cache/qrows_kernels.hip) -----------------------------------------
+ * Not in the reference.  A store of num_rows rows of `dim` values in device memory of the CALLER's:
+ *   codes   num_rows * hps_qrows_row_bytes(dim, bits) bytes; 8 bits: one signed byte per value, 4 bits: two per byte, the
+ *           first in the low half; 4-byte aligned (the rows' last bytes may be padding, written as zeros)
+ *   scales  num_rows * hps_qrows_groups(dim, group) floats; group 0: one scale per row, else one per 16, 32, 64, 128 or 256
+ *           consecutive values (the last group of a row may be shorter)
+ *   owner   num_rows uint32, zero before the first write and left zero by every write
+ * write: per group a = max |x|, scale = fp32(a / L), L = 127 (8 bits) or 7 (4 bits), code = x / scale to the nearest integer,
+ * ties to even; a < 2^-100: scale 0 and codes 0; a NaN or an infinity in the group: scale NaN, so the group reads back as NaN.
+ * A slot outside [0, num_rows) is skipped; of a slot that is named several times in one call the last row stays.
+ * read: out = fp32(code * scale) rounded to `type`; a slot outside [0, num_rows) reads as default_value.
+ * All pointers on `device`, strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
+ * be captured into a graph.  One write at a time per store (`owner` is its workspace); reads beside reads are free. */
+typedef struct hps_qrows {
+  void* codes;
+  float* scales;
+  uint32_t* owner;
+  uint64_t num_rows;
+  uint32_t dim, bits, group;
+} hps_qrows_t;
+uint32_t hps_qrows_row_bytes(uint32_t dim, uint32_t bits);
+uint32_t hps_qrows_groups(uint32_t dim, uint32_t group);
+/* d_rows: [n] rows of `dim` values of `type`, row_stride apart; d_held: null, or where the values that the rows stand for once
+ * they are held (what a later read gives, whether or not the slot keeps them) are written, in `type`, held_stride apart; it may be
+ * d_rows itself. */
+int hps_qrows_write_device(int device, const hps_qrows_t* store, const void* d_rows, int type, uint64_t row_stride,
+                           const int64_t* d_slots, uint64_t n, void* d_held, uint64_t held_stride, void* stream);
+int hps_qrows_read_device(int device, const hps_qrows_t* store, const int64_t* d_slots, uint64_t n, float default_value,
+                          void* d_out, int type, uint64_t out_stride, void* stream);
+
+/* ---- dense layers behind the interaction (csrc/dense/linear_kernels.hip): y = act(x W + b) * mul + residual -----------------
+ * Not in the reference (there the dense model is another Triton backend).  Operands fp16 or bf16 on the matrix cores, sums
+ * and everything behind them in fp32, one rounding at the end.  num_experts > 1: as many layers of one shape, each over its own
+ * run of positions. */
+#define HPS_ACT_NONE 0
+#define HPS_ACT_RELU 1
+#define HPS_ACT_GELU 2      /* with the error function */
+#define HPS_ACT_SILU 3
+#define HPS_ACT_SIGMOID 4
+typedef struct hps_linear hps_linear_t;
+typedef struct hps_linear_args {
+  const void* x;              /* the layer's type, [x_rows] rows x_stride apart (strides in elements) */
+  uint64_t x_stride, x_rows;
+  void* out;                  /* out_type, [out_rows] rows out_stride apart; may be mul or residual itself, else apart from all inputs */
+  uint64_t out_stride, out_rows;
+  int32_t out_type;           /* the layer's type or HPS_TYPE_FP32 */
+  int32_t zero_rest;          /* positions of no run: 0 = their output rows stay as they were, 1 = they become zeros */
+  const void* mul;            /* null, or the layer's type, rows like out's */
+  uint64_t mul_stride;
+  const void* residual;       /* null, or the layer's type, rows like out's */
+  uint64_t residual_stride;
+  uint64_t rows;              /* positions, < 2^31 */
+  const int32_t* offsets;     /* device, [num_experts + 1]: expert e has the positions [offsets[e], offsets[e+1]); may be null for one
+                                 expert (all positions).  Values are clamped to [0, rows] and read as their running maximum */
+  const int32_t* rows_in;     /* null, or device [rows]: the row of x a position reads (outside [0, x_rows): zeros) */
+  const int32_t* rows_out;    /* null, or device [rows]: the row of out, mul and residual it has (outside [0, out_rows): not written);
+                                 a row that several positions name holds, element by element, the result of one of them */
+} hps_linear_args_t;
+/* weights: [num_experts][in_dim][out_dim] row-major (the x @ W convention) of weights_type, rounded to `type`; bias: null or
+ * [num_experts][out_dim] floats.  on_device 0: both in host memory, 1: both on `device`, ready on `stream`.  Synchronises `stream`. */
+int hps_linear_create(int device, uint32_t num_experts, uint32_t in_dim, uint32_t out_dim, int type, int activation,
+                      const void* weights, int weights_type, const float* bias, int on_device, void* stream, hps_linear_t** out);
+void hps_linear_destroy(hps_linear_t* layer);
+/* Enqueued on `stream` (a hipStream_t of the layer's device), not synchronised; any number of calls at once, also captured. */
+int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void* stream);
+/* The runs an expert layer needs: a stable sort of the positions 0 .. n-1 by d_ids[position].  d_offsets[num_experts + 1], d_order[n]:
+ * the positions of expert e are d_order[offsets[e] .. offsets[e+1]); ids outside [0, num_experts) come behind the last run.
+ * n < 2^31, num_experts <= 1024; d_workspace: hps_group_rows_workspace_bytes (may be null where that is 0), one call at a time. */
+uint64_t hps_group_rows_workspace_bytes(uint64_t n, uint32_t num_experts);
+int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t num_experts, int32_t* d_offsets, int32_t* d_order,
+                          void* d_workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
