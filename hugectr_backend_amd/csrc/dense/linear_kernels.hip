@@ -20,7 +20,9 @@ namespace hps {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
 typedef float acc4 __attribute__((ext_vector_type(4)));
+typedef float acc8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u4l __attribute__((ext_vector_type(4)));
+typedef uint32_t u8l __attribute__((ext_vector_type(8)));
 
 template <typename T>
 struct Frag;
@@ -43,21 +45,70 @@ __device__ __forceinline__ u4l load16(const void* p) {
 }
 __device__ __forceinline__ void store16(void* p, u4l v) { __builtin_memcpy(p, &v, 16); }
 
-// erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7): one exponential and a polynomial of degree five
-__device__ __forceinline__ float erf_as(float x) {
-  const float a = fabsf(x), t = 1.f / fmaf(0.3275911f, a, 1.f);
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  return copysignf(fmaf(-p, __expf(-a * a), 1.f), x);
+// the first `left` of eight 2-byte values (all of them from 8 on), the others zero: 4 + 2 + 1 of them, nothing beyond is touched
+__device__ __forceinline__ u4l load_halves(const void* p, uint32_t left) {
+  if (left >= 8) return load16(p);
+  const char* c = reinterpret_cast<const char*>(p);
+  u4l v = {0, 0, 0, 0};
+  if (left & 4) {
+    uint32_t w[2];
+    __builtin_memcpy(w, c, 8);
+    v[0] = w[0], v[1] = w[1];
+  }
+  if (left & 2) {
+    uint32_t w;
+    __builtin_memcpy(&w, c + 2 * (left & 4), 4);
+    if (left & 4) v[2] = w;
+    else v[0] = w;
+  }
+  if (left & 1) {
+    uint16_t h;
+    __builtin_memcpy(&h, c + 2 * (left & 6), 2);
+    if (left == 1) v[0] = h;
+    else if (left == 3) v[1] = h;
+    else if (left == 5) v[2] = h;
+    else v[3] = h;
+  }
+  return v;
 }
 
-__device__ __forceinline__ float activate(float y, int act) {
-  switch (act) {
-    case (int)Activation::kRelu: return y > 0.f ? y : (y != y ? y : 0.f);
-    case (int)Activation::kGelu: return 0.5f * y * (1.f + erf_as(y * 0.70710678f));
-    case (int)Activation::kSilu: return y / (1.f + __expf(-y));
-    case (int)Activation::kSigmoid: return 1.f / (1.f + __expf(-y));
-    default: return y;
+// the first `left` of eight values (all of them from 8 on), of 2 or of 4 bytes
+__device__ __forceinline__ void store_halves(void* p, u4l v, uint32_t left) {
+  if (left >= 8) return store16(p, v);
+  char* c = reinterpret_cast<char*>(p);
+  if (left & 4) {
+    const uint32_t w[2] = {v[0], v[1]};
+    __builtin_memcpy(c, w, 8);
   }
+  if (left & 2) {
+    const uint32_t w = left & 4 ? v[2] : v[0];
+    __builtin_memcpy(c + 2 * (left & 4), &w, 4);
+  }
+  if (left & 1) {
+    const uint16_t h = (uint16_t)(left == 1 ? v[0] : left == 3 ? v[1] : left == 5 ? v[2] : v[3]);
+    __builtin_memcpy(c + 2 * (left & 6), &h, 2);
+  }
+}
+
+__device__ __forceinline__ void store_words(void* p, u8l v, uint32_t left) {
+  char* c = reinterpret_cast<char*>(p);
+  if (left & ~3u) store16(c, u4l{v[0], v[1], v[2], v[3]});
+  if (left >= 8) return store16(c + 16, u4l{v[4], v[5], v[6], v[7]});
+  if (left & 2) {
+    const uint32_t w[2] = {left & 4 ? v[4] : v[0], left & 4 ? v[5] : v[1]};
+    __builtin_memcpy(c + 4 * (left & 4), w, 8);
+  }
+  if (left & 1) {
+    const uint32_t w = left == 1 ? v[0] : left == 3 ? v[2] : left == 5 ? v[4] : v[6];
+    __builtin_memcpy(c + 4 * (left & 6), &w, 4);
+  }
+}
+
+// erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7): one exponential and a polynomial of degree five
+__device__ __forceinline__ float erf_as(float x) {
+  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  return copysignf(fmaf(-p, __expf(-a * a), 1.f), x);
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -146,56 +197,54 @@ __device__ __forceinline__ const T* in_row(const LinearArgs& a, uint32_t pos) {
 // eight values of a row of x from column k on, zeros beyond K and for no row
 template <typename T>
 __device__ __forceinline__ u4l load_x(const T* row, uint32_t k, uint32_t K) {
-  u4l v = {0, 0, 0, 0};
-  if (row == nullptr) return v;
-  if (k + 8 <= K) return load16(row + k);
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (k + j < K) v[j / 2] |= (uint32_t)p[k + j] << (16 * (j % 2));
-  return v;
+  if (row == nullptr || k >= K) return u4l{0, 0, 0, 0};
+  return load_halves(row + k, K - k);
 }
 
-// the end of eight consecutive columns [n, n + 8) of one output row: y = act(acc + bias) * mul + residual, rounded once
+__device__ __forceinline__ acc8 activate(acc8 y, int act) {
+  switch (act) {
+    case (int)Activation::kRelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = __builtin_elementwise_maximum(y[j], 0.f);   // (a NaN stays one)
+      return y;
+    case (int)Activation::kGelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = 0.5f * y[j] * (1.f + erf_as(y[j] * 0.70710678f));
+      return y;
+    // (the hardware's reciprocal is good to one unit in the last place: 2^-23 of results that are rounded to 2^-11 or compared at 2^-20)
+    case (int)Activation::kSilu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * __builtin_amdgcn_rcpf(1.f + __expf(-y[j]));
+      return y;
+    case (int)Activation::kSigmoid:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = __builtin_amdgcn_rcpf(1.f + __expf(-y[j]));
+      return y;
+    default: return y;
+  }
+}
+
+// The end of eight consecutive columns [n, n + 8) of one position of a tile, which may pass N: y = act(y + bias) * mul + residual,
+// rounded once and stored
 template <typename T, typename OutT>
-__device__ __forceinline__ void finish8(const LinearDesc& d, const LinearArgs& a, int64_t row, uint32_t n, const float* __restrict__ bias,
-                                        float (&y)[8]) {
-  if (row < 0 || n >= d.N) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = activate(y[j] + bias[j], d.act);
+__device__ __forceinline__ void finish8(const LinearDesc& d, const LinearArgs& a, const RowTile& t, uint32_t pos, uint32_t n, acc8 bias, acc8 y) {
+  typedef typename Frag<T>::type frag;
+  if (pos >= t.count || n >= d.N) return;
   const uint32_t left = d.N - n;
-  if (a.mul) {
-    const T* m = reinterpret_cast<const T*>(a.mul) + (uint64_t)row * a.mul_stride + n;
-    T v[8];
-    const u4l r = load_x<T>(m, 0, left);
-    __builtin_memcpy(v, &r, 16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] *= (float)v[j];
+  uint64_t row = t.first + pos;
+  if (a.rows_in && (uint64_t)(int64_t)a.rows_in[row] >= a.x_rows) y = acc8{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (a.rows_out) {
+    row = (uint64_t)(int64_t)a.rows_out[row];
+    if (row >= a.out_rows) return;
   }
-  if (a.residual) {
-    const T* m = reinterpret_cast<const T*>(a.residual) + (uint64_t)row * a.residual_stride + n;
-    T v[8];
-    const u4l r = load_x<T>(m, 0, left);
-    __builtin_memcpy(v, &r, 16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] += (float)v[j];
-  }
-  OutT* o = reinterpret_cast<OutT*>(a.out) + (uint64_t)row * a.out_stride + n;
-  if (left >= 8) {
-    OutT v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (OutT)y[j];
-#pragma unroll
-    for (int j = 0; j < (int)sizeof(OutT) / 2; ++j) {
-      u4l r;
-      __builtin_memcpy(&r, reinterpret_cast<const char*>(v) + 16 * j, 16);
-      store16(reinterpret_cast<char*>(o) + 16 * j, r);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if ((uint32_t)j < left) o[j] = (OutT)y[j];
-  }
+  y = activate(y + bias, d.act);
+  if (a.mul)
+    y *= __builtin_convertvector(__builtin_bit_cast(frag, load_halves(reinterpret_cast<const T*>(a.mul) + row * a.mul_stride + n, left)), acc8);
+  if (a.residual)
+    y += __builtin_convertvector(__builtin_bit_cast(frag, load_halves(reinterpret_cast<const T*>(a.residual) + row * a.residual_stride + n, left)), acc8);
+  void* o = reinterpret_cast<OutT*>(a.out) + row * a.out_stride + n;
+  if constexpr (sizeof(OutT) == 4) store_words(o, __builtin_bit_cast(u8l, y), left);
+  else store_halves(o, __builtin_bit_cast(u4l, __builtin_convertvector(y, frag)), left);
 }
 
 template <typename OutT>
@@ -210,60 +259,66 @@ __device__ __forceinline__ void zero_rows(const LinearDesc& d, const LinearArgs&
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Tiles of BM rows x BN columns, WM x WN waves, K in steps of 64.  Both operands go through LDS, double-buffered: the step after next
-// is on its way into registers while the step at hand is multiplied, the next one is written to the other buffer.  Rows of x are 128
-// bytes of LDS, their 16-byte chunks swapped by chunk ^ (row & 7), so that the fragments' reads (16 rows at one chunk) are free of bank
-// conflicts; weight fragments lie in LDS as in memory.
+// Tiles of BM rows x BN columns, WM x WN waves, K in steps of 64, two LDS buffers.  Whole steps go from memory to LDS without passing
+// registers: while a step is multiplied the next one is on its way into the other buffer, one barrier a step.  Rows of x are 128 bytes
+// of LDS, their 16-byte chunks swapped by chunk ^ (row & 7), so that the fragments' reads (16 rows at one chunk) are free of bank
+// conflicts; weight fragments lie in LDS as in memory.  The last step (K not a multiple of 64) and rows that do not start on 16 bytes
+// (ALIGNED false) go through registers, where what lies beyond K becomes zero.
+// Rows beyond the tile's count and positions whose rows_in is outside x read some other row; the former are never stored, the sums of
+// the latter are set to zero in the end.
 // ------------------------------------------------------------------------------------------------------------
-template <typename T, typename OutT, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void to_lds(const void* from, u4l* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <typename T, typename OutT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDesc d, LinearArgs a, uint32_t m_tiles, uint32_t n_tiles) {
-  constexpr int kThreads = 64 * WM * WN;
+  constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FP = BN / WN / 32;     // row fragments and column pairs of a wave
-  constexpr int XC = BM * 8 / kThreads, WC = BN * 8 / kThreads;   // 16-byte chunks of a step per thread
-  static_assert(XC * kThreads == BM * 8 && WC * kThreads == BN * 8 && FM >= 1 && FP >= 1, "whole chunks");
+  constexpr int XC = BM / 8 / kWaves, WC = BN / 8 / kWaves;   // 1-KB pieces (8 rows; a fragment) of a step per wave
+  static_assert(XC * kWaves * 8 == BM && WC * kWaves * 8 == BN && FM >= 1 && FP >= 1, "whole pieces");
   typedef typename Frag<T>::type frag;
-  __shared__ __attribute__((aligned(16))) u4l lds_x[2][BM * 8];
-  __shared__ __attribute__((aligned(16))) u4l lds_w[2][BN * 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) u4l lds[(BM + BN) * 16];
+  u4l *lds_x0 = lds, *lds_x1 = lds + BM * 8, *lds_w0 = lds + BM * 16, *lds_w1 = lds + BM * 16 + BN * 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t id = xcd_order(blockIdx.x, m_tiles * n_tiles);
   const uint32_t nt = id % n_tiles;
   const RowTile t = find_tile<BM>(d, a, id / n_tiles, lane);
   if (t.kind == 0) return;
   if (t.kind == 2) return zero_rows<OutT>(d, a, t, nt * BN, nt * BN + BN);
 
+  const uint32_t chunk = (lane & 7) ^ (lane >> 3);
   const T* xrow[XC];
 #pragma unroll
   for (int i = 0; i < XC; ++i) {
-    const uint32_t r = (uint32_t)(tid >> 3) + i * (kThreads / 8);
-    xrow[i] = r < t.count ? in_row<T>(a, t.first + r) : nullptr;
+    const uint32_t r = (uint32_t)(i * kWaves + wave) * 8 + (lane >> 3);
+    const T* p = in_row<T>(a, t.first + min(r, t.count - 1));
+    xrow[i] = (p ? p : reinterpret_cast<const T*>(a.x)) + chunk * 8;
   }
-  const u4l* wbase = reinterpret_cast<const u4l*>(d.w) + (uint64_t)t.expert * d.npairs * d.ksteps * 128;
-  const u4l* wsrc[WC];
+  const u4l* wsrc[WC];   // (the same for the whole wave)
 #pragma unroll
   for (int i = 0; i < WC; ++i) {
-    const uint32_t q = tid + i * kThreads, p = min(nt * (BN / 32) + (q >> 8), d.npairs - 1);
-    wsrc[i] = wbase + (uint64_t)p * d.ksteps * 128 + (q & 255);
+    const uint32_t q = i * kWaves + wave;     // piece of the step: four fragments per pair
+    const uint32_t p = min(nt * (BN / 32) + (q >> 2), d.npairs - 1);
+    wsrc[i] = reinterpret_cast<const u4l*>(d.w) + ((uint64_t)t.expert * d.npairs + p) * d.ksteps * 128 + (q & 3) * 64;
   }
-  u4l rx[XC], rw[WC];
-  const uint32_t steps = (d.ksteps + 1) / 2;
-  auto fetch = [&](uint32_t s) {
+  u4l rx[XC];
+  auto fetch_w = [&](uint32_t s, u4l* bw) {
 #pragma unroll
-    for (int i = 0; i < XC; ++i) rx[i] = load_x<T>(xrow[i], s * 64 + (tid & 7) * 8, d.K);
-#pragma unroll
-    for (int i = 0; i < WC; ++i) {
-      const uint32_t q = tid + i * kThreads;
-      rw[i] = u4l{0, 0, 0, 0};
-      if (2 * s + ((q >> 7) & 1) < d.ksteps) rw[i] = wsrc[i][(uint64_t)s * 256];
-    }
+    for (int i = 0; i < WC; ++i) to_lds(wsrc[i] + (uint64_t)s * 256 + lane, bw + (i * kWaves + wave) * 64);
   };
-  auto keep = [&](int b) {
+  auto fetch_x = [&](uint32_t s, u4l* bx) {
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
-      const uint32_t r = (uint32_t)(tid >> 3) + i * (kThreads / 8);
-      lds_x[b][r * 8 + ((tid & 7) ^ (r & 7))] = rx[i];
+      if constexpr (ALIGNED) to_lds(xrow[i] + s * 64, bx + (i * kWaves + wave) * 64);
+      else rx[i] = load16(xrow[i] + s * 64);
     }
+  };
+  auto keep_x = [&](u4l* bx) {
+    if constexpr (!ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < WC; ++i) lds_w[b][tid + i * kThreads] = rw[i];
+      for (int i = 0; i < XC; ++i) bx[(i * kWaves + wave) * 64 + lane] = rx[i];
+    }
   };
   const int wm = wave / WN, wn = wave % WN;
   acc4 acc[FP][2][FM];
@@ -273,28 +328,17 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int m = 0; m < FM; ++m) acc[p][h][m] = acc4{0.f, 0.f, 0.f, 0.f};
-
-  fetch(0);
-  keep(0);
-  if (steps > 1) fetch(1);
-  __syncthreads();
-  for (uint32_t s = 0; s < steps; ++s) {
-    const int b = (int)(s & 1);
-    if (s + 1 < steps) keep(b ^ 1);      // (the other buffer was last read before the previous barrier)
-    if (s + 2 < steps) fetch(s + 2);
+  const int xat = wm * FM * 128 + (lane & 15) * 8, wat = wn * FP * 256 + lane;
+  auto multiply = [&](const u4l* bx, const u4l* bw) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       frag fw[FP][2], fx[FM];
 #pragma unroll
       for (int p = 0; p < FP; ++p)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          fw[p][h] = __builtin_bit_cast(frag, lds_w[b][(wn * FP + p) * 256 + ks * 128 + h * 64 + lane]);
+        for (int h = 0; h < 2; ++h) fw[p][h] = __builtin_bit_cast(frag, bw[wat + p * 256 + ks * 128 + h * 64]);
 #pragma unroll
-      for (int m = 0; m < FM; ++m) {
-        const int r = (wm * FM + m) * 16 + (lane & 15);
-        fx[m] = __builtin_bit_cast(frag, lds_x[b][r * 8 + ((ks * 4 + (lane >> 4)) ^ (r & 7))]);
-      }
+      for (int m = 0; m < FM; ++m) fx[m] = __builtin_bit_cast(frag, bx[xat + m * 128 + ((ks * 4 + (lane >> 4)) ^ (lane & 7))]);
 #pragma unroll
       for (int m = 0; m < FM; ++m)
 #pragma unroll
@@ -302,20 +346,140 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
 #pragma unroll
           for (int h = 0; h < 2; ++h) acc[p][h][m] = Frag<T>::mfma(fw[p][h], fx[m], acc[p][h][m]);
     }
-    __syncthreads();
+  };
+  const uint32_t whole = d.K / 64;
+  if (whole) {
+    fetch_w(0, lds_w0);
+    fetch_x(0, lds_x0);
+    keep_x(lds_x0);
   }
-  const float* bias = d.bias + (uint64_t)t.expert * d.npairs * 32;
+  for (uint32_t s = 0; s < whole; s += 2) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's part of step s is in LDS
+    __syncthreads();                      // everybody's is, and nobody reads the other buffer any more
+    if (s + 1 < whole) {
+      fetch_w(s + 1, lds_w1);
+      fetch_x(s + 1, lds_x1);
+    }
+    multiply(lds_x0, lds_w0);
+    if (s + 1 >= whole) break;
+    keep_x(lds_x1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (s + 2 < whole) {
+      fetch_w(s + 2, lds_w0);
+      fetch_x(s + 2, lds_x0);
+    }
+    multiply(lds_x1, lds_w1);
+    if (s + 2 < whole) keep_x(lds_x0);
+  }
+  if (whole * 64 < d.K) {   // the rest of K, into the buffer that nobody reads
+    u4l* bx = whole & 1 ? lds_x1 : lds_x0;
+    u4l* bw = whole & 1 ? lds_w1 : lds_w0;
 #pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    const uint32_t r = (wm * FM + m) * 16 + (lane & 15);
-    const int64_t row = r < t.count ? out_row(a, t.first + r) : -1;
+    for (int i = 0; i < XC; ++i) bx[(i * kWaves + wave) * 64 + lane] = load_x<T>(xrow[i] - chunk * 8, whole * 64 + chunk * 8, d.K);
 #pragma unroll
-    for (int p = 0; p < FP; ++p) {
-      const uint32_t n = nt * BN + (wn * FP + p) * 32 + (lane >> 4) * 8;
-      float y[8];
+    for (int i = 0; i < WC; ++i) {
+      u4l v = {0, 0, 0, 0};
+      if (2 * whole + (((i * kWaves + wave) >> 1) & 1) < d.ksteps) v = wsrc[i][(uint64_t)whole * 256 + lane];
+      bw[(i * kWaves + wave) * 64 + lane] = v;
+    }
+    __syncthreads();
+    multiply(bx, bw);
+  }
+  // The end of the tile.  A vector instruction costs a wave four cycles, 65,536 sums a tile: ten per sum would take as long as 350 of
+  // K.  none and relu over whole tiles of columns (the first branch) take about three, straight from the accumulators: a lane's pair of
+  // fragments is eight consecutive columns of a row, four lanes store 64 bytes of it.
+  constexpr int kCols = FP * 32;
+  const float* const tile_bias = d.bias + (uint64_t)t.expert * d.npairs * 32;
+  if (nt * BN + BN <= d.N && d.act <= (int)Activation::kRelu) {
+    const float floor = d.act == (int)Activation::kRelu ? 0.f : -__builtin_inff();
+    const uint32_t n0 = nt * BN + wn * kCols + (lane >> 4) * 8;
+    acc8 bias[FP];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = acc[p][j / 4][m][j % 4];
-      finish8<T, OutT>(d, a, row, n, bias + n, y);
+    for (int p = 0; p < FP; ++p) bias[p] = *reinterpret_cast<const acc8*>(tile_bias + n0 + p * 32);
+    bool ok[FM], none[FM];
+    uint64_t row[FM];
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      const uint32_t r = (wm * FM + m) * 16 + (lane & 15);
+      ok[m] = r < t.count;
+      row[m] = t.first + (ok[m] ? r : 0u);
+      none[m] = false;
+    }
+    if (a.rows_in) {
+#pragma unroll
+      for (int m = 0; m < FM; ++m) none[m] = (uint64_t)(int64_t)a.rows_in[row[m]] >= a.x_rows;
+    }
+    if (a.rows_out) {
+      int32_t to[FM];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) to[m] = a.rows_out[row[m]];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        const bool inside = (uint64_t)(int64_t)to[m] < a.out_rows;
+        ok[m] = ok[m] && inside;
+        row[m] = inside ? (uint32_t)to[m] : 0u;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      acc8 y[FP];
+#pragma unroll
+      for (int p = 0; p < FP; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[p][j] = __builtin_elementwise_maximum((none[m] ? 0.f : acc[p][j / 4][m][j % 4]) + bias[p][j], floor);
+      if (a.mul) {
+        const T* v = reinterpret_cast<const T*>(a.mul) + row[m] * a.mul_stride + n0;
+#pragma unroll
+        for (int p = 0; p < FP; ++p) y[p] *= __builtin_convertvector(__builtin_bit_cast(frag, load16(v + p * 32)), acc8);
+      }
+      if (a.residual) {
+        const T* v = reinterpret_cast<const T*>(a.residual) + row[m] * a.residual_stride + n0;
+#pragma unroll
+        for (int p = 0; p < FP; ++p) y[p] += __builtin_convertvector(__builtin_bit_cast(frag, load16(v + p * 32)), acc8);
+      }
+      if (ok[m]) {
+        OutT* o = reinterpret_cast<OutT*>(a.out) + row[m] * a.out_stride + n0;
+#pragma unroll
+        for (int p = 0; p < FP; ++p) {
+          if constexpr (sizeof(OutT) == 4) store_words(o + p * 32, __builtin_bit_cast(u8l, y[p]), 8);
+          else store16(o + p * 32, __builtin_bit_cast(u4l, __builtin_convertvector(y[p], frag)));
+        }
+      }
+    }
+    return;
+  }
+  // The other activations, and tiles that pass N: each wave hands its sums through LDS (its own part, kHalf row fragments at a time,
+  // 16-byte chunks swapped by chunk ^ (row & 7)) and takes them back eight columns of a row per lane, so that one short loop does it.
+  constexpr int kLanes = kCols / 8;                                                // lanes that share a row
+  constexpr int kRoom = (BM + BN) * 16 / kWaves;                                    // LDS chunks of a wave
+  constexpr int kHalf = FM * 16 * (kCols / 4) <= kRoom ? FM : FM / 2;              // row fragments at a time
+  constexpr int kIter = kHalf * 16 * kLanes / 64;
+  static_assert(kHalf * 16 * (kCols / 4) <= kRoom && FM % kHalf == 0 && 64 % kLanes == 0, "a wave's sums fit its part of LDS");
+  const uint32_t c8 = lane % kLanes, n = nt * BN + wn * kCols + c8 * 8;
+  // (32 floats per pair of columns: eight from n < N on are there)
+  const acc8 bias = *reinterpret_cast<const acc8*>(tile_bias + (n < d.N ? n : 0));
+  u4l* mine = lds + wave * kRoom;
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  __syncthreads();
+#pragma unroll 1
+  for (int half = 0; half < FM / kHalf; ++half) {
+#pragma unroll
+    for (int m = 0; m < FM; ++m)
+      if (m / kHalf == half)
+#pragma unroll
+        for (int p = 0; p < FP; ++p)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = (m % kHalf) * 16 + (lane & 15), c = p * 8 + (lane >> 4) * 2 + h;
+            mine[r * (kCols / 4) + (c ^ (r & 7))] = __builtin_bit_cast(u4l, acc[p][h][m]);
+          }
+#pragma unroll 1
+    for (int i = 0; i < kIter; ++i) {
+      const int r = i * (64 / kLanes) + lane / kLanes;
+      const u4l* at = mine + r * (kCols / 4);
+      const acc4 v0 = __builtin_bit_cast(acc4, at[(2 * c8) ^ (r & 7)]), v1 = __builtin_bit_cast(acc4, at[(2 * c8 + 1) ^ (r & 7)]);
+      finish8<T, OutT>(d, a, t, (wm * FM + half * kHalf) * 16 + r, n, bias, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 }
@@ -374,16 +538,14 @@ __global__ __launch_bounds__(64 * NW) void hps_linear_rows_kernel(LinearDesc d, 
 #pragma unroll
     for (int m = 0; m < MF; ++m) part[wave][h * MF + m][lane] = acc[h][m];
   __syncthreads();
-  const float* bias = d.bias + ((uint64_t)t.expert * d.npairs + pair) * 32;
+  const float* bias = d.bias + ((uint64_t)t.expert * d.npairs + pair) * 32 + (lane >> 4) * 8;
   for (int m = wave; m < MF; m += NW) {
-    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    acc8 y = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NW; ++v)
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] += part[v][(j / 4) * MF + m][lane][j % 4];
-    const uint32_t r = m * 16 + (lane & 15), n = (lane >> 4) * 8;
-    const int64_t row = r < t.count ? out_row(a, t.first + r) : -1;
-    finish8<T, OutT>(d, a, row, pair * 32 + n, bias + n, y);
+    finish8<T, OutT>(d, a, t, m * 16 + (lane & 15), pair * 32 + (lane >> 4) * 8, *reinterpret_cast<const acc8*>(bias), y);
   }
 }
 
@@ -414,8 +576,9 @@ template <typename T, typename OutT, int BM, int BN, int WM, int WN>
 hipError_t LaunchTile(const LinearDesc& d, const LinearArgs& a, hipStream_t stream) {
   const uint64_t m_tiles = RowTiles(d, a, BM), n_tiles = (d.N + BN - 1) / BN;
   if (m_tiles * n_tiles >= (1ull << 23)) return hipErrorInvalidConfiguration;   // 512 threads each: a launch holds 2^32
-  hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN><<<(uint32_t)(m_tiles * n_tiles), 64 * WM * WN, 0, stream>>>(d, a, (uint32_t)m_tiles,
-                                                                                                             (uint32_t)n_tiles);
+  const bool aligned = (uintptr_t)a.x % 16 == 0 && a.x_stride % 8 == 0;
+  auto* kernel = aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true> : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false>;
+  kernel<<<(uint32_t)(m_tiles * n_tiles), 64 * WM * WN, 0, stream>>>(d, a, (uint32_t)m_tiles, (uint32_t)n_tiles);
   return hipGetLastError();
 }
 
@@ -434,7 +597,7 @@ hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, h
   if (each <= 64) return LaunchRows<T, OutT, 4, 8>(d, a, stream);
   const uint64_t big = (RowTiles(d, a, 256)) * ((d.N + 255) / 256);
   if (d.N > 128 && big >= (uint64_t)cu_count) return LaunchTile<T, OutT, 256, 256, 2, 4>(d, a, stream);
-  return LaunchTile<T, OutT, 128, 128, 2, 2>(d, a, stream);
+  return LaunchTile<T, OutT, 128, 128, 4, 2>(d, a, stream);
 }
 
 template <typename From>
