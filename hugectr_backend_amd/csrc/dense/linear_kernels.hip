@@ -303,15 +303,13 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
     wsrc[i] = reinterpret_cast<const u4l*>(d.w) + ((uint64_t)t.expert * d.npairs + p) * d.ksteps * 128 + (q & 3) * 64;
   }
   u4l rx[XC];
-  auto fetch_w = [&](uint32_t s, u4l* bw) {
-#pragma unroll
-    for (int i = 0; i < WC; ++i) to_lds(wsrc[i] + (uint64_t)s * 256 + lane, bw + (i * kWaves + wave) * 64);
-  };
-  auto fetch_x = [&](uint32_t s, u4l* bx) {
-#pragma unroll
-    for (int i = 0; i < XC; ++i) {
-      if constexpr (ALIGNED) to_lds(xrow[i] + s * 64, bx + (i * kWaves + wave) * 64);
-      else rx[i] = load16(xrow[i] + s * 64);
+  // piece j of step s on its way: the x pieces first, then the weights'
+  auto fetch = [&](int j, uint32_t s, u4l* bx, u4l* bw) {
+    if (j < XC) {
+      if constexpr (ALIGNED) to_lds(xrow[j] + s * 64, bx + (j * kWaves + wave) * 64);
+      else rx[j] = load16(xrow[j] + s * 64);
+    } else {
+      to_lds(wsrc[j - XC] + (uint64_t)s * 256 + lane, bw + ((j - XC) * kWaves + wave) * 64);
     }
   };
   auto keep_x = [&](u4l* bx) {
@@ -329,7 +327,11 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
 #pragma unroll
       for (int m = 0; m < FM; ++m) acc[p][h][m] = acc4{0.f, 0.f, 0.f, 0.f};
   const int xat = wm * FM * 128 + (lane & 15) * 8, wat = wn * FP * 256 + lane;
-  auto multiply = [&](const u4l* bx, const u4l* bw) {
+  // One step.  The pieces of the step `next` (more: there is one) leave between the products, a few at a time: all at once behind the
+  // barrier, every wave waited for the others' copies to be taken before its first product (16384 x 3456 -> 3456: 349 us against 335,
+  // where the raised priority of the products is half of the gain).
+  constexpr int kPieces = XC + WC, kPerRow = (kPieces + 2 * FM - 1) / (2 * FM);
+  auto multiply = [&](const u4l* bx, const u4l* bw, bool more, uint32_t next, u4l* ox, u4l* ow) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       frag fw[FP][2], fx[FM];
@@ -339,38 +341,45 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         for (int h = 0; h < 2; ++h) fw[p][h] = __builtin_bit_cast(frag, bw[wat + p * 256 + ks * 128 + h * 64]);
 #pragma unroll
       for (int m = 0; m < FM; ++m) fx[m] = __builtin_bit_cast(frag, bx[xat + m * 128 + ((ks * 4 + (lane >> 4)) ^ (lane & 7))]);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int m = 0; m < FM; ++m)
+      for (int m = 0; m < FM; ++m) {
 #pragma unroll
         for (int p = 0; p < FP; ++p)
 #pragma unroll
           for (int h = 0; h < 2; ++h) acc[p][h][m] = Frag<T>::mfma(fw[p][h], fx[m], acc[p][h][m]);
+        if (more) {
+#pragma unroll
+          for (int q = 0; q < kPerRow; ++q)
+            if ((ks * FM + m) * kPerRow + q < kPieces) fetch((ks * FM + m) * kPerRow + q, next, ox, ow);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
     }
+    if (more) keep_x(ox);
+  };
+  auto arrived = [&] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's pieces of the step are in LDS
+    __syncthreads();                      // everybody's are, and nobody reads the other buffer any more
   };
   const uint32_t whole = d.K / 64;
   if (whole) {
-    fetch_w(0, lds_w0);
-    fetch_x(0, lds_x0);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) fetch(j, 0, lds_x0, lds_w0);
     keep_x(lds_x0);
-  }
-  for (uint32_t s = 0; s < whole; s += 2) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's part of step s is in LDS
-    __syncthreads();                      // everybody's is, and nobody reads the other buffer any more
+    uint32_t s = 0;
+    for (; s + 2 < whole; s += 2) {
+      arrived();
+      multiply(lds_x0, lds_w0, true, s + 1, lds_x1, lds_w1);
+      arrived();
+      multiply(lds_x1, lds_w1, true, s + 2, lds_x0, lds_w0);
+    }
+    arrived();
+    multiply(lds_x0, lds_w0, s + 1 < whole, s + 1, lds_x1, lds_w1);
     if (s + 1 < whole) {
-      fetch_w(s + 1, lds_w1);
-      fetch_x(s + 1, lds_x1);
+      arrived();
+      multiply(lds_x1, lds_w1, false, 0, lds_x0, lds_w0);
     }
-    multiply(lds_x0, lds_w0);
-    if (s + 1 >= whole) break;
-    keep_x(lds_x1);
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    if (s + 2 < whole) {
-      fetch_w(s + 2, lds_w0);
-      fetch_x(s + 2, lds_x0);
-    }
-    multiply(lds_x1, lds_w1);
-    if (s + 2 < whole) keep_x(lds_x0);
   }
   if (whole * 64 < d.K) {   // the rest of K, into the buffer that nobody reads
     u4l* bx = whole & 1 ? lds_x1 : lds_x0;
@@ -384,7 +393,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
       bw[(i * kWaves + wave) * 64 + lane] = v;
     }
     __syncthreads();
-    multiply(bx, bw);
+    multiply(bx, bw, false, 0, bx, bw);
   }
   // The end of the tile.  A vector instruction costs a wave four cycles, 65,536 sums a tile: ten per sum would take as long as 350 of
   // K.  none and relu over whole tiles of columns (the first branch) take about three, straight from the accumulators: a lane's pair of
@@ -421,22 +430,30 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         row[m] = inside ? (uint32_t)to[m] : 0u;
       }
     }
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      acc8 y[FP];
-#pragma unroll
-      for (int p = 0; p < FP; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[p][j] = __builtin_elementwise_maximum((none[m] ? 0.f : acc[p][j / 4][m][j % 4]) + bias[p][j], floor);
+    frag vm[2][FP], vr[2][FP];   // mul and residual of a row: the next row's are on their way while one is finished
+    auto fetch_row = [&](int m) {
       if (a.mul) {
-        const T* v = reinterpret_cast<const T*>(a.mul) + row[m] * a.mul_stride + n0;
 #pragma unroll
-        for (int p = 0; p < FP; ++p) y[p] *= __builtin_convertvector(__builtin_bit_cast(frag, load16(v + p * 32)), acc8);
+        for (int p = 0; p < FP; ++p)
+          vm[m & 1][p] = __builtin_bit_cast(frag, load16(reinterpret_cast<const T*>(a.mul) + row[m] * a.mul_stride + n0 + p * 32));
       }
       if (a.residual) {
-        const T* v = reinterpret_cast<const T*>(a.residual) + row[m] * a.residual_stride + n0;
 #pragma unroll
-        for (int p = 0; p < FP; ++p) y[p] += __builtin_convertvector(__builtin_bit_cast(frag, load16(v + p * 32)), acc8);
+        for (int p = 0; p < FP; ++p)
+          vr[m & 1][p] = __builtin_bit_cast(frag, load16(reinterpret_cast<const T*>(a.residual) + row[m] * a.residual_stride + n0 + p * 32));
+      }
+    };
+    fetch_row(0);
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      if (m + 1 < FM) fetch_row(m + 1);
+      acc8 y[FP];
+#pragma unroll
+      for (int p = 0; p < FP; ++p) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[p][j] = __builtin_elementwise_maximum((none[m] ? 0.f : acc[p][j / 4][m][j % 4]) + bias[p][j], floor);
+        if (a.mul) y[p] *= __builtin_convertvector(vm[m & 1][p], acc8);
+        if (a.residual) y[p] += __builtin_convertvector(vr[m & 1][p], acc8);
       }
       if (ok[m]) {
         OutT* o = reinterpret_cast<OutT*>(a.out) + row[m] * a.out_stride + n0;
@@ -590,14 +607,20 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
   return hipGetLastError();
 }
 
+// Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
+// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.5 (K = 3456: 27 / 19 / 26); M = 2048: 64 x 64 8.9, 128 x 128 10.9;
+// M = 8192: 128 x 128 20, 256 x 256 32; M = 65536, N = 512: 256 x 256 68, 128 x 128 80.
+// Few columns leave no room for wide tiles: M = 65536, N = 32, K = 128: 64 x 64 5.3, 128 x 128 6.7.
+// With experts the tiles are estimated as half a tile more per expert (the grid has room for the worst case).
 template <typename T, typename OutT>
 hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, hipStream_t stream) {
-  const uint64_t each = a.rows / d.experts;
-  if (each <= 16) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
-  if (each <= 64) return LaunchRows<T, OutT, 4, 8>(d, a, stream);
-  const uint64_t big = (RowTiles(d, a, 256)) * ((d.N + 255) / 256);
-  if (d.N > 128 && big >= (uint64_t)cu_count) return LaunchTile<T, OutT, 256, 256, 2, 4>(d, a, stream);
-  return LaunchTile<T, OutT, 128, 128, 4, 2>(d, a, stream);
+  const uint64_t cus = (uint64_t)cu_count, runs = a.offsets ? (d.experts < a.rows ? d.experts : a.rows) : 0;
+  auto tiles = [&](uint64_t bm, uint64_t bn) { return ((a.rows + bm - 1) / bm + runs / 2) * ((d.N + bn - 1) / bn); };
+  if (tiles(16, 32) <= 2 * cus) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
+  if (tiles(32, 32) <= 2 * cus) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
+  if (tiles(128, 128) < cus || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2>(d, a, stream);
+  if (tiles(256, 256) < cus || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4>(d, a, stream);
+  return LaunchTile<T, OutT, 256, 256, 2, 4>(d, a, stream);
 }
 
 template <typename From>
