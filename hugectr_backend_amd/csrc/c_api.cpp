@@ -816,6 +816,8 @@ uint32_t hps_qrows_row_bytes(uint32_t dim, uint32_t bits) { return QRowsRowBytes
 
 uint32_t hps_qrows_groups(uint32_t dim, uint32_t group) { return group == 0 || group >= dim ? 1u : (dim + group - 1) / group; }
 
+uint64_t hps_qrows_workspace_bytes(uint64_t num_rows) { return QRowsWorkspaceBytes(num_rows); }
+
 namespace {
 Status QRowsStore(const hps_qrows_t* store, bool write, QRowsDesc* d) {
   if (!store) return Error(Code::kInvalidArg, "null argument");
@@ -824,12 +826,14 @@ Status QRowsStore(const hps_qrows_t* store, bool write, QRowsDesc* d) {
   const uint32_t g = store->group;
   if (g != 0 && g != 16 && g != 32 && g != 64 && g != 128 && g != 256)
     return Error(Code::kInvalidArg, "quantised rows: a scale per row (0) or per 16, 32, 64, 128 or 256 values, got ", g);
-  if (store->num_rows && (!store->codes || !store->scales || (write && !store->owner))) return Error(Code::kInvalidArg, "quantised rows: null store pointer");
-  if ((uintptr_t)store->codes % 4 || (uintptr_t)store->scales % 4 || (uintptr_t)store->owner % 4)
-    return Error(Code::kInvalidArg, "quantised rows: codes, scales and owner are 4-byte aligned");
+  if (store->num_rows && (!store->codes || !store->scales || (write && !store->workspace))) return Error(Code::kInvalidArg, "quantised rows: null store pointer");
+  if ((uintptr_t)store->codes % 4 || (uintptr_t)store->scales % 4 || (uintptr_t)store->workspace % 4)
+    return Error(Code::kInvalidArg, "quantised rows: codes, scales and workspace are 4-byte aligned");
   d->codes = (uint8_t*)store->codes;
   d->scales = store->scales;
-  d->owner = store->owner;
+  d->claim = (uint32_t*)store->workspace;
+  d->stamp = d->claim + store->num_rows;
+  d->listed = d->stamp + store->num_rows;
   d->num_rows = store->num_rows;
   d->dim = store->dim;
   d->bits = store->bits;

@@ -15,17 +15,16 @@ class DeviceGuard {
     if (restore_ >= 0) (void)hipSetDevice(restore_);
   }
   Status Enter(int device) {
+    int now = 0;
+    const bool any = hipGetDevice(&now) == hipSuccess;
+    if (any && now == device) return Status::Ok();
     int ndev = 0;
-    if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0)
+    if (!any || hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0)
       return Error(Code::kUnavailable, "this call needs a HIP device and none is visible; there is no CPU fallback");
     if (device < 0 || device >= ndev) return Error(Code::kInvalidArg, "device ", device, " is not visible (", ndev, " HIP devices)");
-    int now = 0;
-    hipError_t e = hipGetDevice(&now);
-    if (e == hipSuccess && now != device) {
-      e = hipSetDevice(device);
-      if (e == hipSuccess) restore_ = now;
-    }
+    const hipError_t e = hipSetDevice(device);
     if (e != hipSuccess) return Error(Code::kInternal, "selecting device ", device, " failed: ", hipGetErrorString(e));
+    restore_ = now;
     return Status::Ok();
   }
 

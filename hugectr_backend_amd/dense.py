@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import hps
-from .quantized_rows import _invalid, elem_type, row_stride
+from .quantized_rows import _invalid, current_stream, elem_type, row_stride
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
@@ -121,11 +121,10 @@ class ExpertLayers:
         self._h = h
 
     def _index(self, t, n, name):
-        import torch
         if t is None:
             return None
-        if not t.is_cuda or t.device.index != self.device or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (
-                n > 1 and t.stride(0) != 1):
+        import torch
+        if t.dtype != torch.int32 or t.get_device() != self.device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
             raise _invalid(f"{name}: a contiguous vector of {n} int32 on cuda:{self.device} expected, got {t.dtype} {tuple(t.shape)} on "
                            f"{t.device}")
         return t.data_ptr()
@@ -146,24 +145,27 @@ class ExpertLayers:
                          self._index(rows_out, rows, "rows_out"), mul, residual, out, out_dtype)
 
     def _run(self, x, rows, offsets, rows_in, rows_out, mul, residual, out, out_dtype):
-        import torch
         if x.dtype != self.dtype:
             raise _invalid(f"x: {self.dtype} expected, got {x.dtype}")
-        a = hps.LinearArgs()
-        a.x_stride, a.x, a.x_rows = row_stride(x, self.in_dim, "x", self.device), x.data_ptr(), x.shape[0]
+        stride = row_stride(x, self.in_dim, "x", self.device)
         if out is None:
-            out = torch.empty((rows, self.out_dim), dtype=out_dtype or self.dtype, device=x.device)
-            a.zero_rest = 1
-        elif out_dtype is not None and out.dtype != out_dtype:
-            raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
-        a.out_stride, a.out, a.out_rows = row_stride(out, self.out_dim, "out", self.device), out.data_ptr(), out.shape[0]
-        a.out_type = elem_type(out.dtype)
+            out = x.new_empty((rows, self.out_dim)) if out_dtype is None else x.new_empty((rows, self.out_dim), dtype=out_dtype)
+            zero_rest, out_stride = 1, self.out_dim
+        else:
+            if out_dtype is not None and out.dtype != out_dtype:
+                raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
+            zero_rest, out_stride = 0, row_stride(out, self.out_dim, "out", self.device)
+        a = hps.LinearArgs(x.data_ptr(), stride, x.shape[0], out.data_ptr(), out_stride, out.shape[0], elem_type(out.dtype), zero_rest)
         if mul is not None:
             a.mul, a.mul_stride = self._beside(mul, out, "mul")
         if residual is not None:
             a.residual, a.residual_stride = self._beside(residual, out, "residual")
-        a.rows, a.offsets, a.rows_in, a.rows_out = rows, offsets, rows_in, rows_out
-        hps._check(hps.LIB.hps_linear_forward(self._h, C.addressof(a), torch.cuda.current_stream(self.device).cuda_stream))
+        a.rows = rows
+        if offsets is not None:
+            a.offsets, a.rows_in, a.rows_out = offsets, rows_in, rows_out
+        rc = hps.LIB.hps_linear_forward(self._h, C.addressof(a), current_stream(self.device))
+        if rc:
+            hps._check(rc)
         return out
 
     def _beside(self, t, out, name):
@@ -204,16 +206,15 @@ def group_rows(ids, num_experts: int):
     order int32 [n]: expert e has the positions order[offsets[e] : offsets[e+1]] in ascending order; positions whose id is outside
     [0, num_experts) come behind the last run.  num_experts <= 1024.  Runs on torch's current stream; may be captured."""
     import torch
-    if not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or (ids.shape[0] > 1 and ids.stride(0) != 1):
+    device = ids.get_device()
+    if device < 0 or ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
         raise _invalid(f"ids: a contiguous CUDA vector of int32 expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
     if not 1 <= num_experts <= 1024:
         raise _invalid(f"grouping: 1..1024 experts supported, got {num_experts}")
     n = ids.shape[0]
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=ids.device)
-    order = torch.empty(n, dtype=torch.int32, device=ids.device)
+    offsets, order = ids.new_empty(num_experts + 1), ids.new_empty(n)
     nbytes = int(hps.LIB.hps_group_rows_workspace_bytes(n, num_experts))
-    work = torch.empty(nbytes, dtype=torch.uint8, device=ids.device) if nbytes else None
-    hps._check(hps.LIB.hps_group_rows_device(ids.device.index, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
-                                             work.data_ptr() if work is not None else None,
-                                             torch.cuda.current_stream(ids.device).cuda_stream))
+    work = ids.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    hps._check(hps.LIB.hps_group_rows_device(device, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
+                                             work.data_ptr() if work is not None else None, current_stream(device)))
     return offsets, order

@@ -85,7 +85,7 @@ class RefreshStats(C.Structure):
 
 
 class QRowsStore(C.Structure):
-    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("owner", C.c_void_p), ("num_rows", C.c_uint64), ("dim", C.c_uint32),
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("workspace", C.c_void_p), ("num_rows", C.c_uint64), ("dim", C.c_uint32),
                 ("bits", C.c_uint32), ("group", C.c_uint32)]
 
 
@@ -195,6 +195,7 @@ def _load() -> C.CDLL:
         "hps_session_lookup_interact_device": (C.c_int, [P, P, P, u64, P, P]),
         "hps_qrows_row_bytes": (u32, [u32, u32]),
         "hps_qrows_groups": (u32, [u32, u32]),
+        "hps_qrows_workspace_bytes": (u64, [u64]),
         "hps_qrows_write_device": (C.c_int, [C.c_int, P, P, C.c_int, u64, P, u64, P, u64, P]),
         "hps_qrows_read_device": (C.c_int, [C.c_int, P, P, u64, C.c_float, P, C.c_int, u64, P]),
         "hps_linear_create": (C.c_int, [C.c_int, u32, u32, u32, C.c_int, C.c_int, P, C.c_int, P, C.c_int, P, C.POINTER(P)]),
@@ -231,7 +232,7 @@ EXPORTED_SYMBOLS = [
     "hps_server_get_shard_cache", "hps_shard_entry_create", "hps_shard_entry_destroy", "hps_shard_entry_lookup",
     "hps_shard_entry_lookup_device", "hps_shard_entry_last_stats", "hps_shard_entry_set_option", "hps_shard_entry_shard_capacity",
     "hps_shard_plan_passes", "hps_multi_gpu_selftest",
-    "hps_qrows_row_bytes", "hps_qrows_groups", "hps_qrows_write_device", "hps_qrows_read_device",
+    "hps_qrows_row_bytes", "hps_qrows_groups", "hps_qrows_workspace_bytes", "hps_qrows_write_device", "hps_qrows_read_device",
     "hps_linear_create", "hps_linear_destroy", "hps_linear_forward", "hps_group_rows_workspace_bytes", "hps_group_rows_device",
 ]
 

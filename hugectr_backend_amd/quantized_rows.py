@@ -13,28 +13,42 @@ def _invalid(msg: str):
     return hps.HpsError(hps.ERR_INVALID_ARG, msg)
 
 
+_ELEM = {}
+
+
 def elem_type(dtype) -> int:
     """HPS_TYPE_* of a torch dtype."""
-    import torch
-    t = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    t = _ELEM.get(dtype)
     if t is None:
-        raise _invalid(f"fp32, fp16 or bf16 values expected, got {dtype}")
+        import torch
+        _ELEM.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        t = _ELEM.get(dtype)
+        if t is None:
+            raise _invalid(f"fp32, fp16 or bf16 values expected, got {dtype}")
     return t
+
+
+def current_stream(device: int) -> int:
+    """The hipStream_t of torch's current stream (without the Stream object around it: 1 us of a 6-us call)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def row_stride(t, width: int, name: str, device: int) -> int:
     """Distance of the rows of a 2-D CUDA tensor on `device` whose values lie side by side, `width` of them per row."""
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise _invalid(f"{name}: a tensor on cuda:{device} expected, got one on {t.device}")
-    if t.dim() != 2 or t.shape[1] != width:
-        raise _invalid(f"{name}: rows of {width} values expected, got shape {tuple(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise _invalid(f"{name}: rows of {width} values expected, got shape {tuple(shape)}")
+    stride = t.stride()
+    if width > 1 and stride[1] != 1:
         raise _invalid(f"{name}: the values of a row have to lie side by side")
-    if t.shape[0] <= 1:
+    if shape[0] <= 1:
         return width
-    if t.stride(0) < width:
-        raise _invalid(f"{name}: the rows overlap (stride {t.stride(0)}, {width} values)")
-    return t.stride(0)
+    if stride[0] < width:
+        raise _invalid(f"{name}: the rows overlap (stride {stride[0]}, {width} values)")
+    return stride[0]
 
 
 class QuantizedRows:
@@ -59,16 +73,15 @@ class QuantizedRows:
         self.codes = torch.zeros((num_rows, int(hps.LIB.hps_qrows_row_bytes(dim, bits))),
                                  dtype=torch.int8 if bits == 8 else torch.uint8, device=dev)
         self.scales = torch.zeros((num_rows, int(hps.LIB.hps_qrows_groups(dim, group))), dtype=torch.float32, device=dev)
-        self._owner = torch.zeros(max(num_rows, 1), dtype=torch.int32, device=dev)
+        self._workspace = torch.zeros(int(hps.LIB.hps_qrows_workspace_bytes(num_rows)) // 4, dtype=torch.int32, device=dev)
         torch.cuda.current_stream(dev).synchronize()      # the store is ready for every stream from here on
-        self._desc = hps.QRowsStore(self.codes.data_ptr(), self.scales.data_ptr(), self._owner.data_ptr(), self.num_rows, self.dim,
+        self._desc = hps.QRowsStore(self.codes.data_ptr(), self.scales.data_ptr(), self._workspace.data_ptr(), self.num_rows, self.dim,
                                     self.bits, self.group)
         self._desc_p = C.addressof(self._desc)
+        self._slot_type = torch.int64
 
     def _slots(self, slots) -> int:
-        import torch
-        if not slots.is_cuda or slots.device.index != self.device or slots.dtype != torch.int64 or slots.dim() != 1 or (
-                slots.shape[0] > 1 and slots.stride(0) != 1):
+        if slots.dtype != self._slot_type or slots.get_device() != self.device or slots.dim() != 1 or not slots.is_contiguous():
             raise _invalid(f"slots: a contiguous vector of int64 on cuda:{self.device} expected, got {slots.dtype} {tuple(slots.shape)} "
                            f"on {slots.device}")
         return slots.shape[0]
@@ -78,7 +91,6 @@ class QuantizedRows:
         skipped, of a slot named several times the last row stays.  held: None, or a tensor like `rows` (or `rows` itself) that takes
         the values the rows stand for once they are held — what read() gives from then on.  Returns `held`.  Runs on torch's
         current stream; may be captured."""
-        import torch
         n = self._slots(slots)
         stride = row_stride(rows, self.dim, "rows", self.device)
         if rows.shape[0] != n:
@@ -90,7 +102,7 @@ class QuantizedRows:
                 raise _invalid(f"held: {n} rows of {rows.dtype} expected, got {held.shape[0]} of {held.dtype}")
             hp = held.data_ptr()
         hps._check(hps.LIB.hps_qrows_write_device(self.device, self._desc_p, rows.data_ptr(), elem_type(rows.dtype), stride,
-                                                  slots.data_ptr(), n, hp, hs, torch.cuda.current_stream(self.device).cuda_stream))
+                                                  slots.data_ptr(), n, hp, hs, current_stream(self.device)))
         return held
 
     def read(self, slots, out=None, dtype=None, default_value: float = 0.0):
@@ -99,12 +111,12 @@ class QuantizedRows:
         import torch
         n = self._slots(slots)
         if out is None:
-            out = torch.empty((n, self.dim), dtype=dtype or torch.float32, device=slots.device)
+            out = slots.new_empty((n, self.dim), dtype=dtype or torch.float32)
         elif dtype is not None and out.dtype != dtype:
             raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
         stride = row_stride(out, self.dim, "out", self.device)
         if out.shape[0] != n:
             raise _invalid(f"out: {n} rows expected, got {out.shape[0]}")
         hps._check(hps.LIB.hps_qrows_read_device(self.device, self._desc_p, slots.data_ptr(), n, default_value, out.data_ptr(),
-                                                 elem_type(out.dtype), stride, torch.cuda.current_stream(self.device).cuda_stream))
+                                                 elem_type(out.dtype), stride, current_stream(self.device)))
         return out

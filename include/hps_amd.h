@@ -455,22 +455,23 @@ int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dens
  *           first in the low half; 4-byte aligned (the rows' last bytes may be padding, written as zeros)
  *   scales  num_rows * hps_qrows_groups(dim, group) floats; group 0: one scale per row, else one per 16, 32, 64, 128 or 256
  *           consecutive values (the last group of a row may be shorter)
- *   owner   num_rows uint32, zero before the first write and left zero by every write
+ *   workspace  hps_qrows_workspace_bytes(num_rows) bytes, zero before the first write, 4-byte aligned; a read needs none
  * write: per group a = max |x|, scale = fp32(a / L), L = 127 (8 bits) or 7 (4 bits), code = x / scale to the nearest integer,
  * ties to even; a < 2^-100: scale 0 and codes 0; a NaN or an infinity in the group: scale NaN, so the group reads back as NaN.
  * A slot outside [0, num_rows) is skipped; of a slot that is named several times in one call the last row stays.
  * read: out = fp32(code * scale) rounded to `type`; a slot outside [0, num_rows) reads as default_value.
  * All pointers on `device`, strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
- * be captured into a graph.  One write at a time per store (`owner` is its workspace); reads beside reads are free. */
+ * be captured into a graph.  One write at a time per store; reads beside reads are free. */
 typedef struct hps_qrows {
   void* codes;
   float* scales;
-  uint32_t* owner;
+  void* workspace;
   uint64_t num_rows;
   uint32_t dim, bits, group;
 } hps_qrows_t;
 uint32_t hps_qrows_row_bytes(uint32_t dim, uint32_t bits);
 uint32_t hps_qrows_groups(uint32_t dim, uint32_t group);
+uint64_t hps_qrows_workspace_bytes(uint64_t num_rows);
 /* d_rows: [n] rows of `dim` values of `type`, row_stride apart; d_held: null, or where the values that the rows stand for once
  * they are held (what a later read gives, whether or not the slot keeps them) are written, in `type`, held_stride apart; it may be
  * d_rows itself. */

@@ -79,7 +79,7 @@ def test_write_and_read_are_exact(n, dim, group, dtype, bits):
     got_c, pad = _unpacked(store)
     assert _same(got_c, want_c) and not pad.any()
     assert _same(store.scales.cpu().numpy(), want_s)
-    assert not store._owner.any()
+    assert not store._workspace[: store.num_rows].any()          # the claims are clear again
     values = torch.from_numpy(_values(codes, scales, group))
     assert torch.equal(held.cpu(), values.to(dt))
     for out_t in (torch.float32, torch.float16, torch.bfloat16):
@@ -128,12 +128,13 @@ def test_ties_borders_and_special_values(bits):
     assert np.isnan(want[len(x) - 5]).sum() == 256          # group 256: the NaN's own group alone
 
 
-@pytest.mark.parametrize("n,dim", [(50, 16), (5000, 4), (20000, 128)])
-def test_a_slot_named_again_keeps_its_last_row(n, dim):
+@pytest.mark.parametrize("n,dim,R", [(50, 16, 7), (2000, 128, 300), (5000, 4, 700), (20000, 128, 3000), (270000, 8, 40000), (300000, 16, 5000000),
+                                     (600000, 3, 10000000), (262144, 5, 3), (270000, 1100, 1000)])
+def test_a_slot_named_again_keeps_its_last_row(n, dim, R):
+    """Few rows, some, many; a few of the slots named twice (the last pass has a list of them), most of them (too many for the list)."""
     import torch
     from hugectr_backend_amd.quantized_rows import QuantizedRows
     rng = np.random.default_rng(n)
-    R = max(3, n // 7)
     x = _rows(rng, n, dim)
     slots = rng.integers(-3, R + 3, n).astype(np.int64)     # some outside the store: skipped
     slots[0], slots[1] = np.iinfo(np.int64).min, np.iinfo(np.int64).max
@@ -141,13 +142,17 @@ def test_a_slot_named_again_keeps_its_last_row(n, dim):
     store.write(torch.from_numpy(_rows(rng, R, dim)).cuda(), torch.arange(R, device="cuda"))
     codes0, scales0 = _unpacked(store)[0], store.scales.cpu().numpy()
     codes, scales = _quantize(x, 8, 0)
-    for i in range(n):
-        if 0 <= slots[i] < R:
-            codes0[slots[i]], scales0[slots[i]] = codes[i], scales[i]
+    last = {s: i for i, s in enumerate(slots.tolist()) if 0 <= s < R}
+    at, of = np.array(list(last)), np.array(list(last.values()))
+    codes0[at], scales0[at] = codes[of], scales[of]
     held = store.write(torch.from_numpy(x).cuda(), torch.from_numpy(slots).cuda(), held=torch.empty(n, dim, device="cuda"))
     assert _same(_unpacked(store)[0], codes0) and _same(store.scales.cpu().numpy(), scales0)
     assert _same(held.cpu().numpy(), _values(codes, scales, 0))     # every row's, kept or not
-    assert not store._owner.any()
+    assert not store._workspace[: store.num_rows].any()          # the claims are clear again
+    rows = torch.from_numpy(x).cuda()          # once more, in place and over what is there
+    assert store.write(rows, torch.from_numpy(slots).cuda(), held=rows) is rows
+    assert _same(rows.cpu().numpy(), _values(codes, scales, 0))
+    assert _same(_unpacked(store)[0], codes0) and _same(store.scales.cpu().numpy(), scales0)
     got = store.read(torch.from_numpy(slots).cuda(), default_value=-2.5).cpu().numpy()
     inside = (slots >= 0) & (slots < R)
     assert _same(got[inside], _values(codes0, scales0, 0)[slots[inside]]) and (got[~inside] == -2.5).all()

@@ -11,7 +11,7 @@ P = 0x10000           # some address; no check follows it
 
 
 def _store(**kw):
-    return hps.QRowsStore(**{**dict(codes=P, scales=P, owner=P, num_rows=100, dim=16, bits=8, group=0), **kw})
+    return hps.QRowsStore(**{**dict(codes=P, scales=P, workspace=P, num_rows=100, dim=16, bits=8, group=0), **kw})
 
 
 def _msg():
@@ -45,7 +45,7 @@ def test_stores_that_cannot_be(kw, word):
 def test_write_and_read_arguments():
     s = _store()
     assert _write(None) == hps.ERR_INVALID_ARG and _read(None) == hps.ERR_INVALID_ARG
-    assert _write(_store(owner=None)) == hps.ERR_INVALID_ARG
+    assert _write(_store(workspace=None)) == hps.ERR_INVALID_ARG
     assert _write(s, type=3) == hps.ERR_INVALID_ARG and "element type" in _msg()
     assert _read(s, type=-1) == hps.ERR_INVALID_ARG
     assert _write(s, rows=None) == hps.ERR_INVALID_ARG and _write(s, slots=None) == hps.ERR_INVALID_ARG
