@@ -224,23 +224,23 @@ __device__ __forceinline__ acc8 activate(acc8 y, int act) {
   }
 }
 
-// The end of eight consecutive columns [n, n + 8) of one position of a tile, which may pass N: y = act(y + bias) * mul + residual,
-// rounded once and stored
-template <typename T, typename OutT>
+// The end of eight consecutive columns [n, n + 8) of one position of a tile, which may pass N: y = act(y) * mul + residual,
+// rounded once and stored; y has its bias, which alone is left for a row of x that is not there
+template <typename T, typename OutT, bool ENDS>
 __device__ __forceinline__ void finish8(const LinearDesc& d, const LinearArgs& a, const RowTile& t, uint32_t pos, uint32_t n, acc8 bias, acc8 y) {
   typedef typename Frag<T>::type frag;
   if (pos >= t.count || n >= d.N) return;
   const uint32_t left = d.N - n;
   uint64_t row = t.first + pos;
-  if (a.rows_in && (uint64_t)(int64_t)a.rows_in[row] >= a.x_rows) y = acc8{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (a.rows_in && (uint64_t)(int64_t)a.rows_in[row] >= a.x_rows) y = bias;
   if (a.rows_out) {
     row = (uint64_t)(int64_t)a.rows_out[row];
     if (row >= a.out_rows) return;
   }
-  y = activate(y + bias, d.act);
-  if (a.mul)
+  y = activate(y, d.act);
+  if (ENDS && a.mul)
     y *= __builtin_convertvector(__builtin_bit_cast(frag, load_halves(reinterpret_cast<const T*>(a.mul) + row * a.mul_stride + n, left)), acc8);
-  if (a.residual)
+  if (ENDS && a.residual)
     y += __builtin_convertvector(__builtin_bit_cast(frag, load_halves(reinterpret_cast<const T*>(a.residual) + row * a.residual_stride + n, left)), acc8);
   void* o = reinterpret_cast<OutT*>(a.out) + row * a.out_stride + n;
   if constexpr (sizeof(OutT) == 4) store_words(o, __builtin_bit_cast(u8l, y), left);
@@ -265,13 +265,14 @@ __device__ __forceinline__ void zero_rows(const LinearDesc& d, const LinearArgs&
 // conflicts; weight fragments lie in LDS as in memory.  The last step (K not a multiple of 64) and rows that do not start on 16 bytes
 // (ALIGNED false) go through registers, where what lies beyond K becomes zero.
 // Rows beyond the tile's count and positions whose rows_in is outside x read some other row; the former are never stored, the sums of
-// the latter are set to zero in the end.
+// the latter are replaced in the end.
 // ------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void to_lds(const void* from, u4l* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-template <typename T, typename OutT, int BM, int BN, int WM, int WN, bool ALIGNED>
+// ENDS: there is mul or residual
+template <typename T, typename OutT, int BM, int BN, int WM, int WN, bool ALIGNED, bool ENDS>
 __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDesc d, LinearArgs a, uint32_t m_tiles, uint32_t n_tiles) {
   constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FP = BN / WN / 32;     // row fragments and column pairs of a wave
@@ -319,13 +320,21 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
     }
   };
   const int wm = wave / WN, wn = wave % WN;
+  // the sums start from the bias (32 floats per pair of columns; pairs beyond N read the last one's and are never stored)
   acc4 acc[FP][2][FM];
+  const float* const tile_bias = d.bias + (uint64_t)t.expert * d.npairs * 32;
+  auto bias_of = [&](int p, int lane) {
+    return *reinterpret_cast<const acc8*>(tile_bias + min(nt * (BN / 32) + wn * FP + p, d.npairs - 1) * 32 + (lane >> 4) * 8);
+  };
 #pragma unroll
-  for (int p = 0; p < FP; ++p)
+  for (int p = 0; p < FP; ++p) {
+    const acc8 b = bias_of(p, lane);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int m = 0; m < FM; ++m) acc[p][h][m] = acc4{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < FM; ++m) {
+      acc[p][0][m] = __builtin_shufflevector(b, b, 0, 1, 2, 3);
+      acc[p][1][m] = __builtin_shufflevector(b, b, 4, 5, 6, 7);
+    }
+  }
   const int xat = wm * FM * 128 + (lane & 15) * 8, wat = wn * FP * 256 + lane;
   // One step.  The pieces of the step `next` (more: there is one) leave between the products, a few at a time: all at once behind the
   // barrier, every wave waited for the others' copies to be taken before its first product (16384 x 3456 -> 3456: 349 us against 335,
@@ -395,29 +404,34 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
     __syncthreads();
     multiply(bx, bw, false, 0, bx, bw);
   }
-  // The end of the tile.  A vector instruction costs a wave four cycles, 65,536 sums a tile: ten per sum would take as long as 350 of
-  // K.  none and relu over whole tiles of columns (the first branch) take about three, straight from the accumulators: a lane's pair of
-  // fragments is eight consecutive columns of a row, four lanes store 64 bytes of it.
+  // (what follows computes its addresses from here: kept from before the loop they would take the sums' registers)
+  int lane_ = lane;
+  asm volatile("" : "+v"(lane_));
+  // The end of the tile.  A vector instruction costs a wave four cycles and a tile has 65,536 sums: ten of them per sum would take as long
+  // as 350 of K.  none and relu over whole tiles of columns take two, straight from the accumulators: a lane's pair of fragments is
+  // eight consecutive columns of a row, four lanes store 64 bytes of it.
   constexpr int kCols = FP * 32;
-  const float* const tile_bias = d.bias + (uint64_t)t.expert * d.npairs * 32;
   if (nt * BN + BN <= d.N && d.act <= (int)Activation::kRelu) {
-    const float floor = d.act == (int)Activation::kRelu ? 0.f : -__builtin_inff();
-    const uint32_t n0 = nt * BN + wn * kCols + (lane >> 4) * 8;
-    acc8 bias[FP];
-#pragma unroll
-    for (int p = 0; p < FP; ++p) bias[p] = *reinterpret_cast<const acc8*>(tile_bias + n0 + p * 32);
-    bool ok[FM], none[FM];
+    const uint32_t n0 = nt * BN + wn * kCols + (lane_ >> 4) * 8;
+    bool ok[FM];
     uint64_t row[FM];
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      const uint32_t r = (wm * FM + m) * 16 + (lane & 15);
+      const uint32_t r = (wm * FM + m) * 16 + (lane_ & 15);
       ok[m] = r < t.count;
       row[m] = t.first + (ok[m] ? r : 0u);
-      none[m] = false;
     }
     if (a.rows_in) {
 #pragma unroll
-      for (int m = 0; m < FM; ++m) none[m] = (uint64_t)(int64_t)a.rows_in[row[m]] >= a.x_rows;
+      for (int m = 0; m < FM; ++m)
+        if ((uint64_t)(int64_t)a.rows_in[row[m]] >= a.x_rows) {
+#pragma unroll
+          for (int p = 0; p < FP; ++p) {
+            const acc8 b = bias_of(p, lane_);
+            acc[p][0][m] = __builtin_shufflevector(b, b, 0, 1, 2, 3);
+            acc[p][1][m] = __builtin_shufflevector(b, b, 4, 5, 6, 7);
+          }
+        }
     }
     if (a.rows_out) {
       int32_t to[FM];
@@ -430,37 +444,64 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         row[m] = inside ? (uint32_t)to[m] : 0u;
       }
     }
-    frag vm[2][FP], vr[2][FP];   // mul and residual of a row: the next row's are on their way while one is finished
-    auto fetch_row = [&](int m) {
-      if (a.mul) {
+    if (d.act == (int)Activation::kRelu) {
 #pragma unroll
-        for (int p = 0; p < FP; ++p)
-          vm[m & 1][p] = __builtin_bit_cast(frag, load16(reinterpret_cast<const T*>(a.mul) + row[m] * a.mul_stride + n0 + p * 32));
-      }
-      if (a.residual) {
+      for (int p = 0; p < FP; ++p)
 #pragma unroll
-        for (int p = 0; p < FP; ++p)
-          vr[m & 1][p] = __builtin_bit_cast(frag, load16(reinterpret_cast<const T*>(a.residual) + row[m] * a.residual_stride + n0 + p * 32));
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[p][h][m][j] = __builtin_elementwise_maximum(acc[p][h][m][j], 0.f);   // (a NaN stays one)
+    }
+    // mul, then residual, each into the accumulators.  Rows in order: the wave's part of the tile is copied to LDS like the rows of x were,
+    // all of it on its way at once and no register taken (loaded a row at a time beside the sums, each row waited for memory:
+    // 16384 x 3456 -> 3456 382 us).  Rows by index, or not on 16 bytes: row by row.  A loop of two turns and one fused multiply-add
+    // (sum * v + 0, then sum * 1 + v: rounded like the product and the sum they are) keep the sums in their registers.
+    if constexpr (ENDS) {
+      constexpr int kPart = FP * 4, kParts = FM * 16 * kPart / 64;   // 16-byte chunks of a row; pieces of 64
+      static_assert(kWaves * FM * 16 * kPart <= (BM + BN) * 16, "the tile fits");
+      u4l* const part = lds + wave * (FM * 16 * kPart);
+      __syncthreads();   // nobody reads the steps' buffers any more
+#pragma unroll 1
+      for (int turn = 0; turn < 2; ++turn) {
+        const T* const base = reinterpret_cast<const T*>(turn ? a.residual : a.mul);
+        const uint64_t stride = turn ? a.residual_stride : a.mul_stride;
+        if (base == nullptr) continue;
+        const bool staged = a.rows_out == nullptr && (uintptr_t)base % 16 == 0 && stride % 8 == 0;
+        if (staged) {
+#pragma unroll 2
+          for (int i = 0; i < kParts; ++i) {
+            const uint32_t q = i * 64 + lane_, r = q / kPart, c = (q % kPart) ^ (r % kPart), at = wm * FM * 16 + r;
+            to_lds(base + (uint64_t)(t.first + (at < t.count ? at : 0u)) * stride + nt * BN + wn * kCols + c * 8, part + i * 64);
+          }
+          __builtin_amdgcn_s_waitcnt(0x0f70);
+        }
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+          for (int p = 0; p < FP; ++p) {
+            const int r = m * 16 + (lane_ & 15), c = p * 4 + (lane_ >> 4);
+            u4l v;
+            if (staged) v = part[r * kPart + (c ^ (r % kPart))];
+            else v = load16(base + row[m] * stride + n0 + p * 32);
+            const acc8 f = __builtin_convertvector(__builtin_bit_cast(frag, v), acc8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              acc[p][j / 4][m][j % 4] = fmaf(acc[p][j / 4][m][j % 4], turn ? 1.f : f[j], turn ? f[j] : 0.f);
+          }
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the next copies come over what has been read
       }
-    };
-    fetch_row(0);
+    }
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      if (m + 1 < FM) fetch_row(m + 1);
-      acc8 y[FP];
-#pragma unroll
-      for (int p = 0; p < FP; ++p) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[p][j] = __builtin_elementwise_maximum((none[m] ? 0.f : acc[p][j / 4][m][j % 4]) + bias[p][j], floor);
-        if (a.mul) y[p] *= __builtin_convertvector(vm[m & 1][p], acc8);
-        if (a.residual) y[p] += __builtin_convertvector(vr[m & 1][p], acc8);
-      }
       if (ok[m]) {
         OutT* o = reinterpret_cast<OutT*>(a.out) + row[m] * a.out_stride + n0;
 #pragma unroll
         for (int p = 0; p < FP; ++p) {
-          if constexpr (sizeof(OutT) == 4) store_words(o + p * 32, __builtin_bit_cast(u8l, y[p]), 8);
-          else store16(o + p * 32, __builtin_bit_cast(u4l, __builtin_convertvector(y[p], frag)));
+          const acc8 y = __builtin_shufflevector(acc[p][0][m], acc[p][1][m], 0, 1, 2, 3, 4, 5, 6, 7);
+          if constexpr (sizeof(OutT) == 4) store_words(o + p * 32, __builtin_bit_cast(u8l, y), 8);
+          else store16(o + p * 32, __builtin_bit_cast(u4l, __builtin_convertvector(y, frag)));
         }
       }
     }
@@ -473,7 +514,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
   constexpr int kHalf = FM * 16 * (kCols / 4) <= kRoom ? FM : FM / 2;              // row fragments at a time
   constexpr int kIter = kHalf * 16 * kLanes / 64;
   static_assert(kHalf * 16 * (kCols / 4) <= kRoom && FM % kHalf == 0 && 64 % kLanes == 0, "a wave's sums fit its part of LDS");
-  const uint32_t c8 = lane % kLanes, n = nt * BN + wn * kCols + c8 * 8;
+  const uint32_t c8 = lane_ % kLanes, n = nt * BN + wn * kCols + c8 * 8;
   // (32 floats per pair of columns: eight from n < N on are there)
   const acc8 bias = *reinterpret_cast<const acc8*>(tile_bias + (n < d.N ? n : 0));
   u4l* mine = lds + wave * kRoom;
@@ -488,15 +529,15 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         for (int p = 0; p < FP; ++p)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = (m % kHalf) * 16 + (lane & 15), c = p * 8 + (lane >> 4) * 2 + h;
+            const int r = (m % kHalf) * 16 + (lane_ & 15), c = p * 8 + (lane_ >> 4) * 2 + h;
             mine[r * (kCols / 4) + (c ^ (r & 7))] = __builtin_bit_cast(u4l, acc[p][h][m]);
           }
 #pragma unroll 1
     for (int i = 0; i < kIter; ++i) {
-      const int r = i * (64 / kLanes) + lane / kLanes;
+      const int r = i * (64 / kLanes) + lane_ / kLanes;
       const u4l* at = mine + r * (kCols / 4);
       const acc4 v0 = __builtin_bit_cast(acc4, at[(2 * c8) ^ (r & 7)]), v1 = __builtin_bit_cast(acc4, at[(2 * c8 + 1) ^ (r & 7)]);
-      finish8<T, OutT>(d, a, t, (wm * FM + half * kHalf) * 16 + r, n, bias, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+      finish8<T, OutT, ENDS>(d, a, t, (wm * FM + half * kHalf) * 16 + r, n, bias, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 }
@@ -557,12 +598,13 @@ __global__ __launch_bounds__(64 * NW) void hps_linear_rows_kernel(LinearDesc d, 
   __syncthreads();
   const float* bias = d.bias + ((uint64_t)t.expert * d.npairs + pair) * 32 + (lane >> 4) * 8;
   for (int m = wave; m < MF; m += NW) {
-    acc8 y = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const acc8 b = *reinterpret_cast<const acc8*>(bias);
+    acc8 y = b;
 #pragma unroll
     for (int v = 0; v < NW; ++v)
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] += part[v][(j / 4) * MF + m][lane][j % 4];
-    finish8<T, OutT>(d, a, t, m * 16 + (lane & 15), pair * 32 + (lane >> 4) * 8, *reinterpret_cast<const acc8*>(bias), y);
+    finish8<T, OutT, true>(d, a, t, m * 16 + (lane & 15), pair * 32 + (lane >> 4) * 8, b, y);
   }
 }
 
@@ -594,7 +636,10 @@ hipError_t LaunchTile(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
   const uint64_t m_tiles = RowTiles(d, a, BM), n_tiles = (d.N + BN - 1) / BN;
   if (m_tiles * n_tiles >= (1ull << 23)) return hipErrorInvalidConfiguration;   // 512 threads each: a launch holds 2^32
   const bool aligned = (uintptr_t)a.x % 16 == 0 && a.x_stride % 8 == 0;
-  auto* kernel = aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true> : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false>;
+  auto* kernel = a.mul || a.residual ? (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true, true>
+                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false, true>)
+                                     : (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true, false>
+                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false, false>);
   kernel<<<(uint32_t)(m_tiles * n_tiles), 64 * WM * WN, 0, stream>>>(d, a, (uint32_t)m_tiles, (uint32_t)n_tiles);
   return hipGetLastError();
 }
