@@ -32,6 +32,7 @@ struct LinearArgs {
   const int32_t* rows_in = nullptr;   // position -> row of x; null: the position itself
   const int32_t* rows_out = nullptr;  // position -> row of out, mul and residual; null: the position itself
   int zero_rest = 0;                  // positions of no run write zeros (else their rows stay as they were)
+  int stream_out = 0;                 // set by the launcher
 };
 
 struct LinearDesc {

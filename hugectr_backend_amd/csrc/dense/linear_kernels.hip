@@ -259,11 +259,14 @@ __device__ __forceinline__ void zero_rows(const LinearDesc& d, const LinearArgs&
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Tiles of BM rows x BN columns, WM x WN waves, K in steps of 64, two LDS buffers.  Whole steps go from memory to LDS without passing
-// registers: while a step is multiplied the next one is on its way into the other buffer, one barrier a step.  Rows of x are 128 bytes
-// of LDS, their 16-byte chunks swapped by chunk ^ (row & 7), so that the fragments' reads (16 rows at one chunk) are free of bank
-// conflicts; weight fragments lie in LDS as in memory.  The last step (K not a multiple of 64) and rows that do not start on 16 bytes
-// (ALIGNED false) go through registers, where what lies beyond K becomes zero.
+// Tiles of BM rows x BN columns, WM x WN waves, K in steps of 32, NB LDS buffers.  Whole steps go from memory to LDS without passing
+// registers, NB - 1 of them on their way at once; one barrier a step.  The widest tile, 128 x 256 with three buffers, is made for two
+// workgroups on a CU: while one waits, starts or ends its tile, the other one's products run (a single 256 x 256 workgroup: 65536 x 479
+// -> 1024 101 us against 80; 65536 rows over 16 experts, 1024 -> 512, 111 against 98).
+// A row of a step is 64 bytes of LDS, its 16-byte chunks swapped by chunk ^ (row / 2 % 4), so that the fragments' reads (16 rows at one
+// chunk) are free of bank conflicts; weight fragments lie in LDS as in memory.  What is left of K below a step comes first, through
+// registers, where what lies beyond K becomes zero: its loads' latency is the first steps' too.  Rows that do not start on 16 bytes
+// (ALIGNED false) go through registers in every step.
 // Rows beyond the tile's count and positions whose rows_in is outside x read some other row; the former are never stored, the sums of
 // the latter are replaced in the end.
 // ------------------------------------------------------------------------------------------------------------
@@ -271,16 +274,30 @@ __device__ __forceinline__ void to_lds(const void* from, u4l* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+// at most n memory operations of this wave left / no LDS operation left; no access moves across
+template <int n>
+__device__ __forceinline__ void wait_memory() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// 16 bytes of an output; a streamed output goes past the caches' usual order
+typedef u4l u4l_anywhere __attribute__((aligned(2)));
+__device__ __forceinline__ void put16(void* p, u4l v, bool stream) {
+  if (stream) __builtin_nontemporal_store(v, reinterpret_cast<u4l_anywhere*>(p));
+  else store16(p, v);
+}
+
 // ENDS: there is mul or residual
-template <typename T, typename OutT, int BM, int BN, int WM, int WN, bool ALIGNED, bool ENDS>
-__global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDesc d, LinearArgs a, uint32_t m_tiles, uint32_t n_tiles) {
+template <typename T, typename OutT, int BM, int BN, int WM, int WN, int NB, bool ALIGNED, bool ENDS>
+__global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(LinearDesc d, LinearArgs a, uint32_t m_tiles, uint32_t n_tiles) {
   constexpr int kWaves = WM * WN;
-  constexpr int FM = BM / WM / 16, FP = BN / WN / 32;     // row fragments and column pairs of a wave
-  constexpr int XC = BM / 8 / kWaves, WC = BN / 8 / kWaves;   // 1-KB pieces (8 rows; a fragment) of a step per wave
-  static_assert(XC * kWaves * 8 == BM && WC * kWaves * 8 == BN && FM >= 1 && FP >= 1, "whole pieces");
+  constexpr int FM = BM / WM / 16, FP = BN / WN / 32;             // row fragments and column pairs of a wave
+  constexpr int XC = BM / 16 / kWaves, WC = BN / 16 / kWaves;     // 1-KB pieces (16 rows; a fragment) of a step per wave
+  static_assert(XC * kWaves * 16 == BM && WC * kWaves * 16 == BN && FM >= 1 && FP >= 1 && NB >= 3, "whole pieces");
+  constexpr int kStage = (BM + BN) * 4;                           // 16-byte chunks of a buffer: the rows', then the weights'
   typedef typename Frag<T>::type frag;
-  __shared__ __attribute__((aligned(16))) u4l lds[(BM + BN) * 16];
-  u4l *lds_x0 = lds, *lds_x1 = lds + BM * 8, *lds_w0 = lds + BM * 16, *lds_w1 = lds + BM * 16 + BN * 8;
+  __shared__ __attribute__((aligned(16))) u4l lds[NB * kStage];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t id = xcd_order(blockIdx.x, m_tiles * n_tiles);
   const uint32_t nt = id % n_tiles;
@@ -288,37 +305,20 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
   if (t.kind == 0) return;
   if (t.kind == 2) return zero_rows<OutT>(d, a, t, nt * BN, nt * BN + BN);
 
-  const uint32_t chunk = (lane & 7) ^ (lane >> 3);
+  const uint32_t chunk = (lane & 3) ^ ((lane >> 3) & 3);          // of row lane / 4 of a piece, the one that belongs where the lane writes
   const T* xrow[XC];
 #pragma unroll
   for (int i = 0; i < XC; ++i) {
-    const uint32_t r = (uint32_t)(i * kWaves + wave) * 8 + (lane >> 3);
+    const uint32_t r = (uint32_t)(i * kWaves + wave) * 16 + (lane >> 2);
     const T* p = in_row<T>(a, t.first + min(r, t.count - 1));
     xrow[i] = (p ? p : reinterpret_cast<const T*>(a.x)) + chunk * 8;
   }
   const u4l* wsrc[WC];   // (the same for the whole wave)
 #pragma unroll
   for (int i = 0; i < WC; ++i) {
-    const uint32_t q = i * kWaves + wave;     // piece of the step: four fragments per pair
-    const uint32_t p = min(nt * (BN / 32) + (q >> 2), d.npairs - 1);
-    wsrc[i] = reinterpret_cast<const u4l*>(d.w) + ((uint64_t)t.expert * d.npairs + p) * d.ksteps * 128 + (q & 3) * 64;
+    const uint32_t q = i * kWaves + wave, p = min(nt * (BN / 32) + (q >> 1), d.npairs - 1);   // fragment of the step, two per pair
+    wsrc[i] = reinterpret_cast<const u4l*>(d.w) + ((uint64_t)t.expert * d.npairs + p) * d.ksteps * 128 + (q & 1) * 64;
   }
-  u4l rx[XC];
-  // piece j of step s on its way: the x pieces first, then the weights'
-  auto fetch = [&](int j, uint32_t s, u4l* bx, u4l* bw) {
-    if (j < XC) {
-      if constexpr (ALIGNED) to_lds(xrow[j] + s * 64, bx + (j * kWaves + wave) * 64);
-      else rx[j] = load16(xrow[j] + s * 64);
-    } else {
-      to_lds(wsrc[j - XC] + (uint64_t)s * 256 + lane, bw + ((j - XC) * kWaves + wave) * 64);
-    }
-  };
-  auto keep_x = [&](u4l* bx) {
-    if constexpr (!ALIGNED) {
-#pragma unroll
-      for (int i = 0; i < XC; ++i) bx[(i * kWaves + wave) * 64 + lane] = rx[i];
-    }
-  };
   const int wm = wave / WN, wn = wave % WN;
   // the sums start from the bias (32 floats per pair of columns; pairs beyond N read the last one's and are never stored)
   acc4 acc[FP][2][FM];
@@ -335,96 +335,126 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
       acc[p][1][m] = __builtin_shufflevector(b, b, 4, 5, 6, 7);
     }
   }
-  const int xat = wm * FM * 128 + (lane & 15) * 8, wat = wn * FP * 256 + lane;
-  // One step.  The pieces of the step `next` (more: there is one) leave between the products, a few at a time: all at once behind the
-  // barrier, every wave waited for the others' copies to be taken before its first product (16384 x 3456 -> 3456: 349 us against 335,
-  // where the raised priority of the products is half of the gain).
-  constexpr int kPieces = XC + WC, kPerRow = (kPieces + 2 * FM - 1) / (2 * FM);
-  auto multiply = [&](const u4l* bx, const u4l* bw, bool more, uint32_t next, u4l* ox, u4l* ow) {
+  const uint32_t whole = d.K / 32;
+  auto copy_x = [&](int i, uint32_t s, u4l* to) { to_lds(xrow[i] + s * 32, to + (i * kWaves + wave) * 64); };
+  auto copy_w = [&](int i, uint32_t s, u4l* to) { to_lds(wsrc[i] + (uint64_t)s * 128 + lane, to + BM * 4 + (i * kWaves + wave) * 64); };
+  u4l rx[XC];
+  auto keep_x = [&](u4l* to) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      frag fw[FP][2], fx[FM];
+    for (int i = 0; i < XC; ++i) to[(i * kWaves + wave) * 64 + lane] = rx[i];
+  };
+  const int xat = wm * FM * 64 + (lane & 15) * 4 + ((lane >> 4) ^ ((lane >> 1) & 3)), wat = BM * 4 + wn * FP * 128 + lane;
+  // One step from buffer b.  The copies of the step NB - 1 later (more) leave between the products, a few at a time: all at once behind the
+  // barrier, every wave would wait for the others' copies to be taken before its first product.  Rows that go through registers leave one
+  // step ahead (one).
+  constexpr int kPieces = XC + WC, kPerRow = (kPieces + FM - 1) / FM;
+  auto multiply = [&](const u4l* b, uint32_t s, bool more, u4l* later, bool one, u4l* next) {
+    frag fw[FP][2], fx[FM];
+#pragma unroll
+    for (int p = 0; p < FP; ++p)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) fw[p][h] = __builtin_bit_cast(frag, b[wat + p * 128 + h * 64]);
+#pragma unroll
+    for (int m = 0; m < FM; ++m) fx[m] = __builtin_bit_cast(frag, b[xat + m * 64]);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
 #pragma unroll
       for (int p = 0; p < FP; ++p)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) fw[p][h] = __builtin_bit_cast(frag, bw[wat + p * 256 + ks * 128 + h * 64]);
+        for (int h = 0; h < 2; ++h) acc[p][h][m] = Frag<T>::mfma(fw[p][h], fx[m], acc[p][h][m]);
 #pragma unroll
-      for (int m = 0; m < FM; ++m) fx[m] = __builtin_bit_cast(frag, bx[xat + m * 128 + ((ks * 4 + (lane >> 4)) ^ (lane & 7))]);
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int m = 0; m < FM; ++m) {
-#pragma unroll
-        for (int p = 0; p < FP; ++p)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) acc[p][h][m] = Frag<T>::mfma(fw[p][h], fx[m], acc[p][h][m]);
-        if (more) {
-#pragma unroll
-          for (int q = 0; q < kPerRow; ++q)
-            if ((ks * FM + m) * kPerRow + q < kPieces) fetch((ks * FM + m) * kPerRow + q, next, ox, ow);
+      for (int q = 0; q < kPerRow; ++q) {
+        const int j = m * kPerRow + q;
+        if (j < XC) {
+          if constexpr (ALIGNED) {
+            if (more) copy_x(j, s + NB - 1, later);
+          } else {
+            if (one) rx[j] = load16(xrow[j] + (s + 1) * 32);
+          }
+        } else if (j < kPieces) {
+          if (more) copy_w(j - XC, s + NB - 1, later);
         }
       }
-      __builtin_amdgcn_s_setprio(0);
     }
-    if (more) keep_x(ox);
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (!ALIGNED) {
+      if (one) keep_x(next);
+    }
   };
-  auto arrived = [&] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's pieces of the step are in LDS
-    __syncthreads();                      // everybody's are, and nobody reads the other buffer any more
-  };
-  const uint32_t whole = d.K / 64;
-  if (whole) {
+  u4l tx[XC], tw[WC];
+  const bool ragged = whole * 32 < d.K;
+  if (ragged) {
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) fetch(j, 0, lds_x0, lds_w0);
-    keep_x(lds_x0);
-    uint32_t s = 0;
-    for (; s + 2 < whole; s += 2) {
-      arrived();
-      multiply(lds_x0, lds_w0, true, s + 1, lds_x1, lds_w1);
-      arrived();
-      multiply(lds_x1, lds_w1, true, s + 2, lds_x0, lds_w0);
-    }
-    arrived();
-    multiply(lds_x0, lds_w0, s + 1 < whole, s + 1, lds_x1, lds_w1);
-    if (s + 1 < whole) {
-      arrived();
-      multiply(lds_x1, lds_w1, false, 0, lds_x0, lds_w0);
+    for (int i = 0; i < XC; ++i) tx[i] = load_x<T>(xrow[i] - chunk * 8, whole * 32 + chunk * 8, d.K);
+#pragma unroll
+    for (int i = 0; i < WC; ++i) tw[i] = wsrc[i][(uint64_t)whole * 128 + lane];
+  }
+  if constexpr (!ALIGNED) {
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < XC; ++i) rx[i] = load16(xrow[i]);
     }
   }
-  if (whole * 64 < d.K) {   // the rest of K, into the buffer that nobody reads
-    u4l* bx = whole & 1 ? lds_x1 : lds_x0;
-    u4l* bw = whole & 1 ? lds_w1 : lds_w0;
 #pragma unroll
-    for (int i = 0; i < XC; ++i) bx[(i * kWaves + wave) * 64 + lane] = load_x<T>(xrow[i] - chunk * 8, whole * 64 + chunk * 8, d.K);
+  for (int q = 0; q < NB - 1; ++q)
+    if ((uint32_t)q < whole) {
+      if constexpr (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < WC; ++i) {
-      u4l v = {0, 0, 0, 0};
-      if (2 * whole + (((i * kWaves + wave) >> 1) & 1) < d.ksteps) v = wsrc[i][(uint64_t)whole * 256 + lane];
-      bw[(i * kWaves + wave) * 64 + lane] = v;
+        for (int i = 0; i < XC; ++i) copy_x(i, q, lds + q * kStage);
+      }
+#pragma unroll
+      for (int i = 0; i < WC; ++i) copy_w(i, q, lds + q * kStage);
     }
+  if constexpr (!ALIGNED) {
+    if (whole) keep_x(lds);
+  }
+  if (ragged) {   // in the last buffer, which the first step's copies take over behind its barrier
+    u4l* b = lds + (NB - 1) * kStage;
+#pragma unroll
+    for (int i = 0; i < XC; ++i) b[(i * kWaves + wave) * 64 + lane] = tx[i];
+#pragma unroll
+    for (int i = 0; i < WC; ++i) b[BM * 4 + (i * kWaves + wave) * 64 + lane] = tw[i];
     __syncthreads();
-    multiply(bx, bw, false, 0, bx, bw);
+    multiply(b, 0, false, b, false, b);
+  }
+  uint32_t s = 0, cur = 0;   // step and its buffer
+  // (in flight behind a step's copies: those of the NB - 2 steps after it)
+  constexpr int kBehind = (ALIGNED ? kPieces : WC) * (NB - 2);
+#pragma unroll 1
+  for (; s + NB - 1 < whole; ++s) {
+    const uint32_t after = cur == NB - 1 ? 0 : cur + 1, before = cur == 0 ? NB - 1 : cur - 1;
+    wait_memory<kBehind>();   // this wave's pieces of the step are in LDS,
+    __syncthreads();          // everybody's are, and nobody reads the buffer before any more
+    multiply(lds + cur * kStage, s, true, lds + before * kStage, true, lds + after * kStage);
+    cur = after;
+  }
+#pragma unroll 1
+  for (; s < whole; ++s) {
+    const uint32_t after = cur == NB - 1 ? 0 : cur + 1;
+    wait_memory<0>();
+    __syncthreads();
+    multiply(lds + cur * kStage, s, false, lds, s + 1 < whole, lds + after * kStage);
+    cur = after;
   }
   // (what follows computes its addresses from here: kept from before the loop they would take the sums' registers)
   int lane_ = lane;
   asm volatile("" : "+v"(lane_));
-  // The end of the tile.  A vector instruction costs a wave four cycles and a tile has 65,536 sums: ten of them per sum would take as long
-  // as 350 of K.  none and relu over whole tiles of columns take two, straight from the accumulators: a lane's pair of fragments is
-  // eight consecutive columns of a row, four lanes store 64 bytes of it.
+  // The end of the tile.  A vector instruction costs a wave four cycles and a tile has 32,768 sums: ten of them per sum would take as long
+  // as 350 of K.  none and relu over whole tiles of columns take two or three, straight from the accumulators.
   constexpr int kCols = FP * 32;
   if (nt * BN + BN <= d.N && d.act <= (int)Activation::kRelu) {
-    const uint32_t n0 = nt * BN + wn * kCols + (lane_ >> 4) * 8;
-    bool ok[FM];
-    uint64_t row[FM];
+    const uint32_t n0 = nt * BN + wn * kCols;
+    uint32_t at[FM];         // the position's output row, ~0: not stored
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
       const uint32_t r = (wm * FM + m) * 16 + (lane_ & 15);
-      ok[m] = r < t.count;
-      row[m] = t.first + (ok[m] ? r : 0u);
+      at[m] = r < t.count ? t.first + r : ~0u;
     }
     if (a.rows_in) {
 #pragma unroll
       for (int m = 0; m < FM; ++m)
-        if ((uint64_t)(int64_t)a.rows_in[row[m]] >= a.x_rows) {
+        if (at[m] != ~0u && (uint64_t)(int64_t)a.rows_in[at[m]] >= a.x_rows) {
 #pragma unroll
           for (int p = 0; p < FP; ++p) {
             const acc8 b = bias_of(p, lane_);
@@ -434,15 +464,12 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         }
     }
     if (a.rows_out) {
-      int32_t to[FM];
 #pragma unroll
-      for (int m = 0; m < FM; ++m) to[m] = a.rows_out[row[m]];
-#pragma unroll
-      for (int m = 0; m < FM; ++m) {
-        const bool inside = (uint64_t)(int64_t)to[m] < a.out_rows;
-        ok[m] = ok[m] && inside;
-        row[m] = inside ? (uint32_t)to[m] : 0u;
-      }
+      for (int m = 0; m < FM; ++m)
+        if (at[m] != ~0u) {
+          const int32_t to = a.rows_out[at[m]];
+          at[m] = (uint64_t)(int64_t)to < a.out_rows ? (uint32_t)to : ~0u;
+        }
     }
     if (d.act == (int)Activation::kRelu) {
 #pragma unroll
@@ -455,12 +482,11 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
             for (int j = 0; j < 4; ++j) acc[p][h][m][j] = __builtin_elementwise_maximum(acc[p][h][m][j], 0.f);   // (a NaN stays one)
     }
     // mul, then residual, each into the accumulators.  Rows in order: the wave's part of the tile is copied to LDS like the rows of x were,
-    // all of it on its way at once and no register taken (loaded a row at a time beside the sums, each row waited for memory:
-    // 16384 x 3456 -> 3456 382 us).  Rows by index, or not on 16 bytes: row by row.  A loop of two turns and one fused multiply-add
-    // (sum * v + 0, then sum * 1 + v: rounded like the product and the sum they are) keep the sums in their registers.
+    // all of it on its way at once and no register taken.  Rows by index, or not on 16 bytes: row by row.  A loop of two turns and one
+    // fused multiply-add (sum * v + 0, then sum * 1 + v: rounded like the product and the sum they are) keep the sums in their registers.
     if constexpr (ENDS) {
       constexpr int kPart = FP * 4, kParts = FM * 16 * kPart / 64;   // 16-byte chunks of a row; pieces of 64
-      static_assert(kWaves * FM * 16 * kPart <= (BM + BN) * 16, "the tile fits");
+      static_assert(kWaves * FM * 16 * kPart <= NB * kStage, "the tile fits");
       u4l* const part = lds + wave * (FM * 16 * kPart);
       __syncthreads();   // nobody reads the steps' buffers any more
 #pragma unroll 1
@@ -472,37 +498,57 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
         if (staged) {
 #pragma unroll 2
           for (int i = 0; i < kParts; ++i) {
-            const uint32_t q = i * 64 + lane_, r = q / kPart, c = (q % kPart) ^ (r % kPart), at = wm * FM * 16 + r;
-            to_lds(base + (uint64_t)(t.first + (at < t.count ? at : 0u)) * stride + nt * BN + wn * kCols + c * 8, part + i * 64);
+            const uint32_t q = i * 64 + lane_, r = q / kPart, c = (q % kPart) ^ (r % kPart), pos = wm * FM * 16 + r;
+            to_lds(base + (uint64_t)(t.first + (pos < t.count ? pos : 0u)) * stride + n0 + c * 8, part + i * 64);
           }
-          __builtin_amdgcn_s_waitcnt(0x0f70);
+          wait_memory<0>();
         }
 #pragma unroll
         for (int m = 0; m < FM; ++m)
 #pragma unroll
           for (int p = 0; p < FP; ++p) {
             const int r = m * 16 + (lane_ & 15), c = p * 4 + (lane_ >> 4);
-            u4l v;
+            u4l v = {0, 0, 0, 0};
             if (staged) v = part[r * kPart + (c ^ (r % kPart))];
-            else v = load16(base + row[m] * stride + n0 + p * 32);
+            else if (at[m] != ~0u) v = load16(base + (uint64_t)at[m] * stride + n0 + c * 8);
             const acc8 f = __builtin_convertvector(__builtin_bit_cast(frag, v), acc8);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               acc[p][j / 4][m][j % 4] = fmaf(acc[p][j / 4][m][j % 4], turn ? 1.f : f[j], turn ? f[j] : 0.f);
           }
-        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the next copies come over what has been read
+        wait_lds();   // the next copies come over what has been read
       }
     }
+    // A lane has eight consecutive columns of a row in every pair.  Two 16-byte chunks of row r (two pairs, or a pair's halves in fp32) are
+    // exchanged with the lane of row r ^ 8, so that a store writes 128 consecutive bytes of eight rows instead of 64 of sixteen.
+    const bool high = (lane_ & 8) != 0, stream = a.stream_out != 0;
+    auto put_two = [&](uint32_t m, u4l q0, u4l q1, uint32_t c0, uint32_t c1) {
+      u4l low, up;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(high ? q0[j] : q1[j]), 0x128, 0xf, 0xf, false);   // row_ror:8
+        low[j] = high ? got : q0[j];
+        up[j] = high ? q1[j] : got;
+      }
+      const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)at[m], 0x128, 0xf, 0xf, false);
+      const uint32_t rl = high ? other : at[m], ru = high ? at[m] : other, c = high ? c1 : c0;
+      if (rl != ~0u) put16(reinterpret_cast<OutT*>(a.out) + (uint64_t)rl * a.out_stride + c, low, stream);
+      if (ru != ~0u) put16(reinterpret_cast<OutT*>(a.out) + (uint64_t)ru * a.out_stride + c, up, stream);
+    };
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      if (ok[m]) {
-        OutT* o = reinterpret_cast<OutT*>(a.out) + row[m] * a.out_stride + n0;
+      const uint32_t c = n0 + (lane_ >> 4) * 8;
+      if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-        for (int p = 0; p < FP; ++p) {
-          const acc8 y = __builtin_shufflevector(acc[p][0][m], acc[p][1][m], 0, 1, 2, 3, 4, 5, 6, 7);
-          if constexpr (sizeof(OutT) == 4) store_words(o + p * 32, __builtin_bit_cast(u8l, y), 8);
-          else store16(o + p * 32, __builtin_bit_cast(u4l, __builtin_convertvector(y, frag)));
-        }
+        for (int p = 0; p < FP; ++p)
+          put_two(m, __builtin_bit_cast(u4l, acc[p][0][m]), __builtin_bit_cast(u4l, acc[p][1][m]), c + p * 32, c + p * 32 + 4);
+      } else {
+        u4l q[FP];
+#pragma unroll
+        for (int p = 0; p < FP; ++p)
+          q[p] = __builtin_bit_cast(u4l, __builtin_convertvector(__builtin_shufflevector(acc[p][0][m], acc[p][1][m], 0, 1, 2, 3, 4, 5, 6, 7), frag));
+        if constexpr (FP == 2) put_two(m, q[0], q[1], c, c + 32);
+        else if (at[m] != ~0u) put16(reinterpret_cast<OutT*>(a.out) + (uint64_t)at[m] * a.out_stride + c, q[0], stream);
       }
     }
     return;
@@ -510,15 +556,15 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
   // The other activations, and tiles that pass N: each wave hands its sums through LDS (its own part, kHalf row fragments at a time,
   // 16-byte chunks swapped by chunk ^ (row & 7)) and takes them back eight columns of a row per lane, so that one short loop does it.
   constexpr int kLanes = kCols / 8;                                                // lanes that share a row
-  constexpr int kRoom = (BM + BN) * 16 / kWaves;                                    // LDS chunks of a wave
+  constexpr int kRoom = NB * kStage / kWaves;                                       // LDS chunks of a wave
   constexpr int kHalf = FM * 16 * (kCols / 4) <= kRoom ? FM : FM / 2;              // row fragments at a time
   constexpr int kIter = kHalf * 16 * kLanes / 64;
   static_assert(kHalf * 16 * (kCols / 4) <= kRoom && FM % kHalf == 0 && 64 % kLanes == 0, "a wave's sums fit its part of LDS");
+  static_assert(FP <= 2, "two pairs of columns are stored together");
   const uint32_t c8 = lane_ % kLanes, n = nt * BN + wn * kCols + c8 * 8;
   // (32 floats per pair of columns: eight from n < N on are there)
   const acc8 bias = *reinterpret_cast<const acc8*>(tile_bias + (n < d.N ? n : 0));
   u4l* mine = lds + wave * kRoom;
-  __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 #pragma unroll 1
   for (int half = 0; half < FM / kHalf; ++half) {
@@ -535,8 +581,8 @@ __global__ __launch_bounds__(64 * WM * WN) void hps_linear_tile_kernel(LinearDes
 #pragma unroll 1
     for (int i = 0; i < kIter; ++i) {
       const int r = i * (64 / kLanes) + lane_ / kLanes;
-      const u4l* at = mine + r * (kCols / 4);
-      const acc4 v0 = __builtin_bit_cast(acc4, at[(2 * c8) ^ (r & 7)]), v1 = __builtin_bit_cast(acc4, at[(2 * c8 + 1) ^ (r & 7)]);
+      const u4l* row = mine + r * (kCols / 4);
+      const acc4 v0 = __builtin_bit_cast(acc4, row[(2 * c8) ^ (r & 7)]), v1 = __builtin_bit_cast(acc4, row[(2 * c8 + 1) ^ (r & 7)]);
       finish8<T, OutT, ENDS>(d, a, t, (wm * FM + half * kHalf) * 16 + r, n, bias, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -631,15 +677,15 @@ __global__ __launch_bounds__(256) void hps_linear_pack_kernel(const From* __rest
 
 namespace {
 
-template <typename T, typename OutT, int BM, int BN, int WM, int WN>
+template <typename T, typename OutT, int BM, int BN, int WM, int WN, int NB>
 hipError_t LaunchTile(const LinearDesc& d, const LinearArgs& a, hipStream_t stream) {
   const uint64_t m_tiles = RowTiles(d, a, BM), n_tiles = (d.N + BN - 1) / BN;
   if (m_tiles * n_tiles >= (1ull << 23)) return hipErrorInvalidConfiguration;   // 512 threads each: a launch holds 2^32
   const bool aligned = (uintptr_t)a.x % 16 == 0 && a.x_stride % 8 == 0;
-  auto* kernel = a.mul || a.residual ? (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true, true>
-                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false, true>)
-                                     : (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, true, false>
-                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, false, false>);
+  auto* kernel = a.mul || a.residual ? (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, true, true>
+                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, true>)
+                                     : (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, true, false>
+                                                : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, false>);
   kernel<<<(uint32_t)(m_tiles * n_tiles), 64 * WM * WN, 0, stream>>>(d, a, (uint32_t)m_tiles, (uint32_t)n_tiles);
   return hipGetLastError();
 }
@@ -652,10 +698,14 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
   return hipGetLastError();
 }
 
+// An output larger than the L2s together (32 MB) leaves by streaming stores: it would push out x and the weights, which the other tiles
+// still read.  65536 x 479 -> 1024 (134 MB) 103 -> 80 us, 16384 x 1024 -> 1024 (34 MB) 33 -> 32; a smaller one may stay for its reader.
+constexpr uint64_t kStreamBytes = 32ull << 20;
+
 // Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
-// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.5 (K = 3456: 27 / 19 / 26); M = 2048: 64 x 64 8.9, 128 x 128 10.9;
-// M = 8192: 128 x 128 20, 256 x 256 32; M = 65536, N = 512: 256 x 256 68, 128 x 128 80.
-// Few columns leave no room for wide tiles: M = 65536, N = 32, K = 128: 64 x 64 5.3, 128 x 128 6.7.
+// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6; M = 2048: 64 x 64 9.1, 128 x 128 11.4; M = 8192: 64 x 64 31, 128 x
+// 128 21.6, 128 x 256 21.3; M = 65536, N = K = 256: 128 x 128 17.0, 128 x 256 15.6.  Few columns leave no room for wide tiles: M = 65536,
+// N = 64, K = 256: 64 x 64 9.2, 128 x 128 11.1.
 // With experts the tiles are estimated as half a tile more per expert (the grid has room for the worst case).
 template <typename T, typename OutT>
 hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, hipStream_t stream) {
@@ -663,9 +713,9 @@ hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, h
   auto tiles = [&](uint64_t bm, uint64_t bn) { return ((a.rows + bm - 1) / bm + runs / 2) * ((d.N + bn - 1) / bn); };
   if (tiles(16, 32) <= 2 * cus) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
   if (tiles(32, 32) <= 2 * cus) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
-  if (tiles(128, 128) < cus || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2>(d, a, stream);
-  if (tiles(256, 256) < cus || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4>(d, a, stream);
-  return LaunchTile<T, OutT, 256, 256, 2, 4>(d, a, stream);
+  if (tiles(128, 128) < cus || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
+  if (tiles(128, 256) < cus || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
+  return LaunchTile<T, OutT, 128, 256, 2, 4, 3>(d, a, stream);
 }
 
 template <typename From>
@@ -687,7 +737,9 @@ hipError_t LaunchLinearPack(const void* d_w, ElemType from, uint32_t experts, ui
   return PackFrom<__bf16>(d_w, experts, K, N, d_packed, to, stream);
 }
 
-hipError_t LaunchLinear(const LinearDesc& d, const LinearArgs& a, ElemType type, ElemType out_type, int cu_count, hipStream_t stream) {
+hipError_t LaunchLinear(const LinearDesc& d, const LinearArgs& args, ElemType type, ElemType out_type, int cu_count, hipStream_t stream) {
+  LinearArgs a = args;
+  a.stream_out = a.rows * d.N * ElemBytes(out_type) >= kStreamBytes;
   if (type == ElemType::kF16)
     return out_type == ElemType::kF32 ? LaunchTyped<_Float16, float>(d, a, cu_count, stream)
                                       : LaunchTyped<_Float16, _Float16>(d, a, cu_count, stream);
