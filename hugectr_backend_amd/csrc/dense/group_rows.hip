@@ -3,8 +3,9 @@
 //
 //   hps_group_rows_one     up to kOneBlockRows positions: one block does everything
 //   hps_group_rows_count   ids per (expert, block of kGroupTile positions)
-//   hps_group_rows_scan    one block: start of every (expert, block), the offsets
-//   hps_group_rows_place   positions to their places
+//   hps_group_rows_scan    one block per expert: where every block's ids of it start within its run
+//   hps_group_rows_place   positions to their places; up to kFewTiles blocks it sums the counts itself (one launch less: 65,536 ids
+//                          over 16 experts 14.9 -> 12.6 us with the call's own costs)
 //
 // Within a block a wave takes 64 consecutive positions; the lanes with the same id find each other with one ballot per bit of the id,
 // so a position's place is start + lanes below it + earlier waves' counts: no atomics on the way, the order never varies.
@@ -20,6 +21,7 @@ constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr uint32_t kGroupTile = kGroupThreads;
 constexpr uint32_t kGroupBins = kMaxExperts + 1;   // the last one in use: ids of no expert
 constexpr uint32_t kOneBlockRows = 8192;
+constexpr uint32_t kFewTiles = 64;                 // a wave's lanes hold one expert's counts
 
 __device__ __forceinline__ uint32_t bin_of(int32_t id, uint32_t experts) { return id >= 0 && (uint32_t)id < experts ? (uint32_t)id : experts; }
 
@@ -141,6 +143,8 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_scan(uint32_t ti
   if (threadIdx.x == 0) total[blockIdx.x] = before;
 }
 
+// SCANNED: counts and total are the scan's; else counts are plain and tiles <= kFewTiles
+template <bool SCANNED>
 __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_place(const int32_t* __restrict__ ids, uint64_t n, uint32_t experts,
                                                                       uint32_t bits, uint32_t tiles, const uint32_t* __restrict__ counts,
                                                                       const uint32_t* __restrict__ total, int32_t* __restrict__ offsets,
@@ -148,16 +152,36 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_place(const int3
   __shared__ uint32_t next[kGroupBins + 1];
   __shared__ uint16_t in_wave[kGroupWaves][kGroupBins];
   __shared__ uint32_t carry[kGroupWaves];
+  __shared__ uint32_t sums[SCANNED ? 1 : kGroupBins + 1];
   const uint32_t bins = experts + 1;
   const uint32_t i0 = 2 * threadIdx.x, i1 = i0 + 1;
+  if constexpr (!SCANNED) {
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t bin = threadIdx.x >> 6; bin < bins; bin += kGroupWaves) {
+      const uint32_t c = lane < tiles ? counts[(uint64_t)bin * tiles + lane] : 0;
+      uint32_t all = c, before = lane < blockIdx.x ? c : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        all += (uint32_t)__shfl_xor((int)all, d, 64);
+        before += (uint32_t)__shfl_xor((int)before, d, 64);
+      }
+      if (lane == 0) {
+        sums[bin] = all;
+        next[bin] = before;
+      }
+    }
+    __syncthreads();
+  }
+  auto total_of = [&](uint32_t i) { return i >= bins ? 0u : SCANNED ? total[i] : sums[i]; };
+  auto before_of = [&](uint32_t i) { return SCANNED ? counts[(uint64_t)i * tiles + blockIdx.x] : next[i]; };
   uint32_t a, b;
-  block_scan2(i0 < bins ? total[i0] : 0, i1 < bins ? total[i1] : 0, carry, a, b);
+  block_scan2(total_of(i0), total_of(i1), carry, a, b);
   if (i0 < bins) {
-    next[i0] = a + counts[(uint64_t)i0 * tiles + blockIdx.x];
+    next[i0] = a + before_of(i0);
     if (blockIdx.x == 0) offsets[i0] = (int32_t)a;
   }
   if (i1 < bins) {
-    next[i1] = b + counts[(uint64_t)i1 * tiles + blockIdx.x];
+    next[i1] = b + before_of(i1);
     if (blockIdx.x == 0) offsets[i1] = (int32_t)b;
   }
   __syncthreads();
@@ -182,8 +206,12 @@ hipError_t LaunchGroupRows(const int32_t* d_ids, uint64_t n, uint32_t experts, i
   uint32_t* counts = (uint32_t*)d_workspace;
   uint32_t* total = counts + (uint64_t)(experts + 1) * tiles;
   hps_group_rows_count<<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, tiles, counts);
+  if (tiles <= kFewTiles) {
+    hps_group_rows_place<false><<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
+    return hipGetLastError();
+  }
   hps_group_rows_scan<<<experts + 1, kGroupThreads, 0, stream>>>(tiles, counts, total);
-  hps_group_rows_place<<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
+  hps_group_rows_place<true><<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
   return hipGetLastError();
 }
 
