@@ -288,6 +288,8 @@ __device__ __forceinline__ void put16(void* p, u4l v, bool stream) {
   else store16(p, v);
 }
 
+constexpr uint32_t kBand = 8;
+
 // ENDS: there is mul or residual
 template <typename T, typename OutT, int BM, int BN, int WM, int WN, int NB, bool ALIGNED, bool ENDS>
 __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(LinearDesc d, LinearArgs a, uint32_t m_tiles, uint32_t n_tiles) {
@@ -299,9 +301,10 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
   typedef typename Frag<T>::type frag;
   __shared__ __attribute__((aligned(16))) u4l lds[NB * kStage];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t id = xcd_order(blockIdx.x, m_tiles * n_tiles);
-  const uint32_t nt = id % n_tiles;
-  const RowTile t = find_tile<BM>(d, a, id / n_tiles, lane);
+  // bands of kBand row tiles, column by column: the 64 workgroups an XCD holds at once read 8 x 8 tiles' operands, not 5 x 14
+  const uint32_t id = xcd_order(blockIdx.x, m_tiles * n_tiles), band = id / (kBand * n_tiles), in_band = id - band * kBand * n_tiles;
+  const uint32_t high_of = min(kBand, m_tiles - band * kBand), nt = in_band / high_of;
+  const RowTile t = find_tile<BM>(d, a, band * kBand + in_band % high_of, lane);
   if (t.kind == 0) return;
   if (t.kind == 2) return zero_rows<OutT>(d, a, t, nt * BN, nt * BN + BN);
 
@@ -320,6 +323,8 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
     wsrc[i] = reinterpret_cast<const u4l*>(d.w) + ((uint64_t)t.expert * d.npairs + p) * d.ksteps * 128 + (q & 1) * 64;
   }
   const int wm = wave / WN, wn = wave % WN;
+  const uint32_t n0 = nt * BN + wn * FP * 32;                     // the wave's first column
+  const bool idle = n0 >= d.N || (uint32_t)(wm * FM * 16) >= t.count;   // nothing of the wave's is stored: it only copies
   // the sums start from the bias (32 floats per pair of columns; pairs beyond N read the last one's and are never stored)
   acc4 acc[FP][2][FM];
   const float* const tile_bias = d.bias + (uint64_t)t.expert * d.npairs * 32;
@@ -348,7 +353,26 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
   // barrier, every wave would wait for the others' copies to be taken before its first product.  Rows that go through registers leave one
   // step ahead (one).
   constexpr int kPieces = XC + WC, kPerRow = (kPieces + FM - 1) / FM;
+  auto leave = [&](int j, uint32_t s, bool more, u4l* later, bool one) {
+    if (j < XC) {
+      if constexpr (ALIGNED) {
+        if (more) copy_x(j, s + NB - 1, later);
+      } else {
+        if (one) rx[j] = load16(xrow[j] + (s + 1) * 32);
+      }
+    } else if (j < kPieces) {
+      if (more) copy_w(j - XC, s + NB - 1, later);
+    }
+  };
   auto multiply = [&](const u4l* b, uint32_t s, bool more, u4l* later, bool one, u4l* next) {
+    if (idle) {
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) leave(j, s, more, later, one);
+      if constexpr (!ALIGNED) {
+        if (one) keep_x(next);
+      }
+      return;
+    }
     frag fw[FP][2], fx[FM];
 #pragma unroll
     for (int p = 0; p < FP; ++p)
@@ -364,18 +388,7 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
 #pragma unroll
         for (int h = 0; h < 2; ++h) acc[p][h][m] = Frag<T>::mfma(fw[p][h], fx[m], acc[p][h][m]);
 #pragma unroll
-      for (int q = 0; q < kPerRow; ++q) {
-        const int j = m * kPerRow + q;
-        if (j < XC) {
-          if constexpr (ALIGNED) {
-            if (more) copy_x(j, s + NB - 1, later);
-          } else {
-            if (one) rx[j] = load16(xrow[j] + (s + 1) * 32);
-          }
-        } else if (j < kPieces) {
-          if (more) copy_w(j - XC, s + NB - 1, later);
-        }
-      }
+      for (int q = 0; q < kPerRow; ++q) leave(m * kPerRow + q, s, more, later, one);
     }
     __builtin_amdgcn_s_setprio(0);
     if constexpr (!ALIGNED) {
@@ -441,10 +454,13 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
   int lane_ = lane;
   asm volatile("" : "+v"(lane_));
   // The end of the tile.  A vector instruction costs a wave four cycles and a tile has 32,768 sums: ten of them per sum would take as long
-  // as 350 of K.  none and relu over whole tiles of columns take two or three, straight from the accumulators.
+  // as 350 of K.  none and relu over a wave's whole columns take two or three, straight from the accumulators.
   constexpr int kCols = FP * 32;
-  if (nt * BN + BN <= d.N && d.act <= (int)Activation::kRelu) {
-    const uint32_t n0 = nt * BN + wn * kCols;
+  constexpr int kRoom = NB * kStage / kWaves;   // LDS chunks of a wave, its own from here on
+  u4l* const mine = lds + wave * kRoom;
+  __syncthreads();                              // nobody reads the steps' buffers any more
+  if (idle) return;
+  if (n0 + kCols <= d.N && d.act <= (int)Activation::kRelu) {
     uint32_t at[FM];         // the position's output row, ~0: not stored
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
@@ -486,9 +502,7 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
     // fused multiply-add (sum * v + 0, then sum * 1 + v: rounded like the product and the sum they are) keep the sums in their registers.
     if constexpr (ENDS) {
       constexpr int kPart = FP * 4, kParts = FM * 16 * kPart / 64;   // 16-byte chunks of a row; pieces of 64
-      static_assert(kWaves * FM * 16 * kPart <= NB * kStage, "the tile fits");
-      u4l* const part = lds + wave * (FM * 16 * kPart);
-      __syncthreads();   // nobody reads the steps' buffers any more
+      static_assert(FM * 16 * kPart <= kRoom, "the wave's part of the tile fits");
 #pragma unroll 1
       for (int turn = 0; turn < 2; ++turn) {
         const T* const base = reinterpret_cast<const T*>(turn ? a.residual : a.mul);
@@ -499,7 +513,7 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
 #pragma unroll 2
           for (int i = 0; i < kParts; ++i) {
             const uint32_t q = i * 64 + lane_, r = q / kPart, c = (q % kPart) ^ (r % kPart), pos = wm * FM * 16 + r;
-            to_lds(base + (uint64_t)(t.first + (pos < t.count ? pos : 0u)) * stride + n0 + c * 8, part + i * 64);
+            to_lds(base + (uint64_t)(t.first + (pos < t.count ? pos : 0u)) * stride + n0 + c * 8, mine + i * 64);
           }
           wait_memory<0>();
         }
@@ -509,7 +523,7 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
           for (int p = 0; p < FP; ++p) {
             const int r = m * 16 + (lane_ & 15), c = p * 4 + (lane_ >> 4);
             u4l v = {0, 0, 0, 0};
-            if (staged) v = part[r * kPart + (c ^ (r % kPart))];
+            if (staged) v = mine[r * kPart + (c ^ (r % kPart))];
             else if (at[m] != ~0u) v = load16(base + (uint64_t)at[m] * stride + n0 + c * 8);
             const acc8 f = __builtin_convertvector(__builtin_bit_cast(frag, v), acc8);
 #pragma unroll
@@ -553,19 +567,16 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
     }
     return;
   }
-  // The other activations, and tiles that pass N: each wave hands its sums through LDS (its own part, kHalf row fragments at a time,
+  // The other activations, and columns that pass N: each wave hands its sums through LDS (its own part, kHalf row fragments at a time,
   // 16-byte chunks swapped by chunk ^ (row & 7)) and takes them back eight columns of a row per lane, so that one short loop does it.
   constexpr int kLanes = kCols / 8;                                                // lanes that share a row
-  constexpr int kRoom = NB * kStage / kWaves;                                       // LDS chunks of a wave
   constexpr int kHalf = FM * 16 * (kCols / 4) <= kRoom ? FM : FM / 2;              // row fragments at a time
   constexpr int kIter = kHalf * 16 * kLanes / 64;
   static_assert(kHalf * 16 * (kCols / 4) <= kRoom && FM % kHalf == 0 && 64 % kLanes == 0, "a wave's sums fit its part of LDS");
   static_assert(FP <= 2, "two pairs of columns are stored together");
-  const uint32_t c8 = lane_ % kLanes, n = nt * BN + wn * kCols + c8 * 8;
+  const uint32_t c8 = lane_ % kLanes, n = n0 + c8 * 8;
   // (32 floats per pair of columns: eight from n < N on are there)
   const acc8 bias = *reinterpret_cast<const acc8*>(tile_bias + (n < d.N ? n : 0));
-  u4l* mine = lds + wave * kRoom;
-  __syncthreads();
 #pragma unroll 1
   for (int half = 0; half < FM / kHalf; ++half) {
 #pragma unroll
