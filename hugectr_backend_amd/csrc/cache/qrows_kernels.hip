@@ -13,7 +13,8 @@
 // multiply-add gives exactly (rounding a nonzero number never changes its sign, and 2^-100 keeps it out of the denormals).
 //
 // A slot that is named twice in one call keeps its LAST row, whole.  Three ways, by the number of rows:
-//   few (kScan)     a row's team looks for its slot among the later ones itself: one launch
+//   few (kScan)     one launch: a block keeps its rows' slots in a table in LDS and reads the slots behind them, which leave the last
+//                   position of each there
 //   some (kClaim)   a first kernel leaves the highest position in claim[slot] with one atomic maximum per row; a row is written where its
 //                   own position is there, and puts the zero back, so the array is clear for the next call (or a graph's next replay)
 //   many (kStamp)   1.7 M atomics are 65 us, 1.7 M plain stores 23: a first kernel stores the positions into stamp[slot], any one of a
@@ -35,7 +36,8 @@ typedef uint32_t u4q __attribute__((ext_vector_type(4)));
 
 constexpr int kQThreads = 256;
 constexpr uint64_t kQRowsPerLaunch = 1ull << 24;   // a launch holds at most 2^32 threads; a row takes up to 64
-constexpr uint32_t kQScanSteps = 64;
+// calls of kScan against kClaim, rows of 16: 1,024 rows 5.1 us, 2,048 5.6 against 8.0, 4,096 8.7 against 8.0
+constexpr uint64_t kScanRows = 2048;
 constexpr float kQTiny = 0x1p-100f;
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -113,6 +115,54 @@ __global__ __launch_bounds__(kQThreads) void hps_qrows_stamp_kernel(const int64_
   if (slot >= 0 && (uint64_t)slot < num_rows) stamp[slot] = (uint32_t)i + 1u;
 }
 
+// The last position + 1 that names `slot` (of this team's row, at position mine - 1; `insert` on the lane that enters it), for a block whose
+// per_block teams hold consecutive rows.  Eight times as many places as rows: a wave searches as long as its unluckiest lane.
+__device__ __forceinline__ uint32_t last_of(const int64_t* __restrict__ slots, uint64_t n, uint64_t num_rows, uint32_t per_block, int64_t slot,
+                                            bool insert, uint32_t mine, uint32_t lane) {
+  constexpr unsigned long long kFree = ~0ull;   // (no slot: the highest bit)
+  __shared__ unsigned long long key[8 * kQThreads];
+  __shared__ uint32_t last[8 * kQThreads];
+  const uint32_t mask = 8 * per_block - 1;
+  auto place = [&](int64_t k) { return (uint32_t)(((uint64_t)k * 0x9E3779B97F4A7C15ull) >> 40) & mask; };
+  for (uint32_t i = threadIdx.x; i <= mask; i += kQThreads) {
+    key[i] = kFree;
+    last[i] = 0;
+  }
+  __syncthreads();
+  uint32_t at = place(slot);
+  if (insert) {
+    for (;;) {
+      const unsigned long long was = atomicCAS(&key[at], kFree, (unsigned long long)slot);
+      if (was == kFree || was == (unsigned long long)slot) break;
+      at = (at + 1) & mask;
+    }
+    atomicMax(&last[at], mine);
+  }
+  __syncthreads();
+  constexpr int kEach = 4;
+  for (uint64_t base = (uint64_t)(blockIdx.x + 1) * per_block; base < n; base += kQThreads * kEach) {
+    int64_t k[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const uint64_t j = base + (uint64_t)e * kQThreads + threadIdx.x;
+      k[e] = j < n ? slots[j] : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (k[e] < 0 || (uint64_t)k[e] >= num_rows) continue;
+      for (uint32_t p = place(k[e]); key[p] != kFree; p = (p + 1) & mask)
+        if (key[p] == (unsigned long long)k[e]) {
+          atomicMax(&last[p], (uint32_t)(base + (uint64_t)e * kQThreads + threadIdx.x) + 1u);
+          break;
+        }
+    }
+  }
+  __syncthreads();
+  // the place belongs to the team's lane 0; the teams' lanes share a wave
+  const uint32_t found = insert ? last[at] : 0u;
+  return (uint32_t)__shfl((int)found, (int)((threadIdx.x & 63) - lane), 64);
+}
+
 constexpr int kScan = 0, kClaim = 1, kStamp = 2, kListed = 3;
 constexpr uint32_t kRaised = 0x80000000u;
 
@@ -185,10 +235,8 @@ __global__ __launch_bounds__(kQThreads) void hps_qrows_write_kernel(QRowsDesc s,
     for (int u = 0; u < U; ++u) {
       const uint32_t me = (uint32_t)row[u] + 1u;
       if constexpr (MODE == kScan) {
-        int again = 0;
-        for (uint64_t j = row[u] + 1 + lane; j < n; j += team) again |= slots[j] == slot[u];
-        for (uint32_t d = 1; d < team; d <<= 1) again |= __shfl_xor(again, (int)d, 64);
-        mine[u] = mine[u] && !again;
+        const uint32_t last = last_of(slots, n, s.num_rows, per_block, slot[u], mine[u] && lane == 0, me, lane);   // (the whole block)
+        mine[u] = mine[u] && last == me;
       } else if constexpr (MODE == kListed) {
         mine[u] = mine[u] && seen[u] == (kRaised | me);
       } else {
@@ -380,7 +428,7 @@ hipError_t WriteKept(const QRowsDesc& s, const T* rows, uint64_t row_stride, con
     return (uint32_t)((rows_of + per - 1) / per);
   };
   auto flat = [&](uint64_t each) { return (uint32_t)((n + (uint64_t)kQThreads * each - 1) / ((uint64_t)kQThreads * each)); };
-  if (n <= ((uint64_t)kQScanSteps << t.team_log)) {
+  if (n <= kScanRows) {
     hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kScan><<<blocks(n, 1), kQThreads, 0, stream>>>(s, rows, row_stride, slots, 0, n, held, held_stride,
                                                                                              t.team_log, t.reduce_lanes);
     return hipGetLastError();

@@ -128,7 +128,7 @@ def test_ties_borders_and_special_values(bits):
     assert np.isnan(want[len(x) - 5]).sum() == 256          # group 256: the NaN's own group alone
 
 
-@pytest.mark.parametrize("n,dim,R", [(50, 16, 7), (2000, 128, 300), (5000, 4, 700), (20000, 128, 3000), (270000, 8, 40000), (300000, 16, 5000000),
+@pytest.mark.parametrize("n,dim,R", [(50, 16, 7), (300, 1, 2), (1000, 1, 400), (2000, 128, 300), (20000, 16, 9000), (26624, 16, 1000000), (40000, 1, 30000), (5000, 4, 700), (20000, 128, 3000), (270000, 8, 40000), (300000, 16, 5000000),
                                      (600000, 3, 10000000), (262144, 5, 3), (270000, 1100, 1000)])
 def test_a_slot_named_again_keeps_its_last_row(n, dim, R):
     """Few rows, some, many; a few of the slots named twice (the last pass has a list of them), most of them (too many for the list)."""
