@@ -45,63 +45,55 @@ __device__ __forceinline__ u4l load16(const void* p) {
 }
 __device__ __forceinline__ void store16(void* p, u4l v) { __builtin_memcpy(p, &v, 16); }
 
-// the first `left` of eight 2-byte values (all of them from 8 on), the others zero: 4 + 2 + 1 of them, nothing beyond is touched
+// The first `left` of eight values (all of them from 8 on), the others zero: 4 + 2 + 1 of them, nothing beyond is touched.  What is
+// loaded or stored is picked by selects alone: as a chain of branches the compiler left the case of seven values unset.
 __device__ __forceinline__ u4l load_halves(const void* p, uint32_t left) {
   if (left >= 8) return load16(p);
   const char* c = reinterpret_cast<const char*>(p);
-  u4l v = {0, 0, 0, 0};
-  if (left & 4) {
-    uint32_t w[2];
-    __builtin_memcpy(w, c, 8);
-    v[0] = w[0], v[1] = w[1];
-  }
-  if (left & 2) {
-    uint32_t w;
-    __builtin_memcpy(&w, c + 2 * (left & 4), 4);
-    if (left & 4) v[2] = w;
-    else v[0] = w;
-  }
+  uint32_t four[2] = {0, 0}, two = 0, one = 0;
+  if (left & 4) __builtin_memcpy(four, c, 8);
+  if (left & 2) __builtin_memcpy(&two, c + 2 * (left & 4), 4);
   if (left & 1) {
     uint16_t h;
     __builtin_memcpy(&h, c + 2 * (left & 6), 2);
-    if (left == 1) v[0] = h;
-    else if (left == 3) v[1] = h;
-    else if (left == 5) v[2] = h;
-    else v[3] = h;
+    one = h;
   }
+  // word j has values 2 j and 2 j + 1
+  u4l v = {four[0], four[1], 0, 0};
+  v[0] |= left & 4 ? 0u : two;
+  v[2] |= left & 4 ? two : 0u;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) v[j] |= (left >> 1) == j ? one : 0u;
   return v;
 }
 
-// the first `left` of eight values (all of them from 8 on), of 2 or of 4 bytes
+// the first `left` of eight values, of 2 or of 4 bytes
 __device__ __forceinline__ void store_halves(void* p, u4l v, uint32_t left) {
   if (left >= 8) return store16(p, v);
   char* c = reinterpret_cast<char*>(p);
-  if (left & 4) {
-    const uint32_t w[2] = {v[0], v[1]};
-    __builtin_memcpy(c, w, 8);
-  }
-  if (left & 2) {
-    const uint32_t w = left & 4 ? v[2] : v[0];
-    __builtin_memcpy(c + 2 * (left & 4), &w, 4);
-  }
-  if (left & 1) {
-    const uint16_t h = (uint16_t)(left == 1 ? v[0] : left == 3 ? v[1] : left == 5 ? v[2] : v[3]);
-    __builtin_memcpy(c + 2 * (left & 6), &h, 2);
-  }
+  uint32_t two = left & 4 ? v[2] : v[0], one = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) one |= (left >> 1) == j ? v[j] : 0u;
+  const uint32_t four[2] = {v[0], v[1]};
+  const uint16_t h = (uint16_t)one;
+  if (left & 4) __builtin_memcpy(c, four, 8);
+  if (left & 2) __builtin_memcpy(c + 2 * (left & 4), &two, 4);
+  if (left & 1) __builtin_memcpy(c + 2 * (left & 6), &h, 2);
 }
 
 __device__ __forceinline__ void store_words(void* p, u8l v, uint32_t left) {
   char* c = reinterpret_cast<char*>(p);
-  if (left & ~3u) store16(c, u4l{v[0], v[1], v[2], v[3]});
-  if (left >= 8) return store16(c + 16, u4l{v[4], v[5], v[6], v[7]});
-  if (left & 2) {
-    const uint32_t w[2] = {left & 4 ? v[4] : v[0], left & 4 ? v[5] : v[1]};
-    __builtin_memcpy(c + 4 * (left & 4), w, 8);
+  if (left >= 8) {
+    store16(c, u4l{v[0], v[1], v[2], v[3]});
+    return store16(c + 16, u4l{v[4], v[5], v[6], v[7]});
   }
-  if (left & 1) {
-    const uint32_t w = left == 1 ? v[0] : left == 3 ? v[2] : left == 5 ? v[4] : v[6];
-    __builtin_memcpy(c + 4 * (left & 6), &w, 4);
-  }
+  const uint32_t two[2] = {left & 4 ? v[4] : v[0], left & 4 ? v[5] : v[1]};
+  uint32_t one = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) one |= (left >> 1) == j ? v[2 * j] : 0u;
+  if (left & 4) store16(c, u4l{v[0], v[1], v[2], v[3]});
+  if (left & 2) __builtin_memcpy(c + 4 * (left & 4), two, 8);
+  if (left & 1) __builtin_memcpy(c + 4 * (left & 6), &one, 4);
 }
 
 // erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7): one exponential and a polynomial of degree five

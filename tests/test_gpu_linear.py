@@ -119,6 +119,27 @@ def test_activation_mul_and_residual(act, m, dtype):
     assert torch.equal(r, layer.forward(x, mul=mul, residual=res))
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m", [5, 100, 400])
+def test_every_width_below_and_beyond_eight(m, dtype):
+    """K and N of every residue modulo 8 (the last values of a row are loaded and stored 4 + 2 + 1), in every kernel, with mul and
+    residual, into both output types: the outputs between sentinels, the rows of x next to each other."""
+    import torch
+    from hugectr_backend_amd.dense import LinearLayer
+    dt = getattr(torch, dtype)
+    for n in list(range(1, 17)) + [31, 39, 47, 61, 69, 77, 127, 131]:
+        k = n if n < 17 else 2 * n
+        x, w, b = _operands(torch, m, k, n, dt, n)
+        mul, res = _operands(torch, m, n, 1, dt, n + 1)[0], _operands(torch, m, n, 1, dt, n + 2)[0]
+        for act in ("relu", "silu"):
+            layer = LinearLayer(w[0], b[0], activation=act, dtype=dt)
+            for out_t in (dt, torch.float32):
+                wide = torch.full((m, n + 3), 77.0, dtype=out_t, device="cuda")
+                layer.forward(x, mul=mul, residual=res, out=wide[:, 1: 1 + n])
+                _check(wide[:, 1: 1 + n], x, w[0], b[0], act, mul, res)
+                assert (wide[:, 0] == 77).all() and (wide[:, 1 + n:] == 77).all()
+
+
 def test_activations_far_out_stay_finite():
     """Sums of +-60000: no exponential overflows into a NaN."""
     import torch
