@@ -4,8 +4,7 @@
 //   hps_group_rows_one     up to kOneBlockRows positions: one block does everything
 //   hps_group_rows_count   ids per (expert, block of kGroupTile positions)
 //   hps_group_rows_scan    one block per expert: where every block's ids of it start within its run
-//   hps_group_rows_place   positions to their places; up to kFewTiles blocks it sums the counts itself (one launch less: 65,536 ids
-//                          over 16 experts 14.9 -> 12.6 us with the call's own costs)
+//   hps_group_rows_place   positions to their places; while the counts are few it sums them itself, one launch less
 //
 // Within a block a wave takes 64 consecutive positions; the lanes with the same id find each other with one ballot per bit of the id,
 // so a position's place is start + lanes below it + earlier waves' counts: no atomics on the way, the order never varies.
@@ -20,8 +19,9 @@ constexpr int kGroupThreads = 1024;
 constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr uint32_t kGroupTile = kGroupThreads;
 constexpr uint32_t kGroupBins = kMaxExperts + 1;   // the last one in use: ids of no expert
-constexpr uint32_t kOneBlockRows = 8192;
-constexpr uint32_t kFewTiles = 64;                 // a wave's lanes hold one expert's counts
+constexpr uint32_t kOneBlockRows = 4096;   // whole calls, one launch / two: 4,096 ids 7.3-10.2 us / 10.6-11.5, 8,192 12.2-18.2 / 10.5-11.6
+constexpr uint32_t kFewTiles = 64;
+constexpr uint32_t kFewCounts = 12288;     // summed by every block, or scanned: 8,500 counts 11.0 / 13.3 us, 12,300 13.1 / 13.2, 43,000 23.9 / 17.1
 
 __device__ __forceinline__ uint32_t bin_of(int32_t id, uint32_t experts) { return id >= 0 && (uint32_t)id < experts ? (uint32_t)id : experts; }
 
@@ -55,39 +55,45 @@ __device__ __forceinline__ void block_scan2(uint32_t va, uint32_t vb, uint32_t* 
   __syncthreads();
 }
 
-// Places of one tile: next[bin] is the first free place of every bin and is advanced behind the tile.
+// What the first `waves` waves of the tile hold of one bin: pairs of 16-bit counts are added as words (a tile has 1,024 ids)
+__device__ __forceinline__ uint32_t count_of_waves(const uint16_t* counts, int waves) {
+  const uint4 lo = *reinterpret_cast<const uint4*>(counts), hi = *reinterpret_cast<const uint4*>(counts + 8);
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += 2 * i + 1 < waves ? w[i] : 2 * i < waves ? w[i] & 0xffff : 0;
+  return (sum & 0xffff) + (sum >> 16);
+}
+
+// Places of one tile: next[bin] is the first free place of every bin; with ADVANCE the call moves it behind the tile.
+// in_wave[bin][wave]: the tile's ids.
+template <bool ADVANCE>
 __device__ __forceinline__ void place_tile(const int32_t* __restrict__ ids, uint64_t n, uint64_t base, uint32_t experts, uint32_t bits,
-                                           uint32_t* next, uint16_t (*in_wave)[kGroupBins], int32_t* __restrict__ order) {
+                                           uint32_t* next, uint16_t (*in_wave)[kGroupWaves], int32_t* __restrict__ order) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t bins = experts + 1;
-  for (uint32_t i = threadIdx.x; i < bins * kGroupWaves; i += kGroupThreads) in_wave[i / bins][i % bins] = 0;
-  __syncthreads();
   const uint64_t at = base + threadIdx.x;
   const bool live = at < n;
   const uint32_t bin = live ? bin_of(ids[at], experts) : experts;
+  for (uint32_t i = threadIdx.x; i < bins * kGroupWaves / 8; i += kGroupThreads) reinterpret_cast<uint4*>(in_wave)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
   const uint64_t same = same_bin(bin, live, bits);
   const uint32_t below = (uint32_t)__popcll(same & ((1ull << lane) - 1));
-  if (live && below == 0) in_wave[wave][bin] = (uint16_t)__popcll(same);
+  if (live && below == 0) in_wave[bin][wave] = (uint16_t)__popcll(same);
   __syncthreads();
-  if (live) {
-    uint32_t p = next[bin] + below;
-    for (int w = 0; w < wave; ++w) p += in_wave[w][bin];
-    order[p] = (int32_t)at;
+  if (live) order[next[bin] + below + count_of_waves(in_wave[bin], wave)] = (int32_t)at;
+  if constexpr (ADVANCE) {
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) next[b] += count_of_waves(in_wave[b], kGroupWaves);
+    __syncthreads();
   }
-  __syncthreads();
-  for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) {
-    uint32_t c = 0;
-    for (int w = 0; w < kGroupWaves; ++w) c += in_wave[w][b];
-    next[b] += c;
-  }
-  __syncthreads();
 }
 
 __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_one(const int32_t* __restrict__ ids, uint32_t n, uint32_t experts,
                                                                     uint32_t bits, int32_t* __restrict__ offsets,
                                                                     int32_t* __restrict__ order) {
   __shared__ uint32_t next[kGroupBins + 1];
-  __shared__ uint16_t in_wave[kGroupWaves][kGroupBins];
+  __shared__ __attribute__((aligned(16))) uint16_t in_wave[kGroupBins][kGroupWaves];
   __shared__ uint32_t carry[kGroupWaves];
   const uint32_t bins = experts + 1;
   for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) next[b] = 0;
@@ -106,11 +112,11 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_one(const int32_
     offsets[i1] = (int32_t)b;
   }
   __syncthreads();
-  for (uint32_t base = 0; base < n; base += kGroupTile) place_tile(ids, n, base, experts, bits, next, in_wave, order);
+  for (uint32_t base = 0; base < n; base += kGroupTile) place_tile<true>(ids, n, base, experts, bits, next, in_wave, order);
 }
 
 __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_count(const int32_t* __restrict__ ids, uint64_t n, uint32_t experts,
-                                                                      uint32_t tiles, uint32_t* __restrict__ counts) {
+                                                                      uint64_t of_bin, uint64_t of_tile, uint32_t* __restrict__ counts) {
   __shared__ uint32_t hist[kGroupBins];
   const uint32_t bins = experts + 1;
   for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) hist[b] = 0;
@@ -118,7 +124,7 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_count(const int3
   const uint64_t at = (uint64_t)blockIdx.x * kGroupTile + threadIdx.x;
   if (at < n) atomicAdd(&hist[bin_of(ids[at], experts)], 1u);
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) counts[(uint64_t)b * tiles + blockIdx.x] = hist[b];
+  for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) counts[b * of_bin + blockIdx.x * of_tile] = hist[b];
 }
 
 // counts[bin][tile] becomes the tile's first place within the bin; total[bin] its sum.  One block per bin.
@@ -143,32 +149,35 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_scan(uint32_t ti
   if (threadIdx.x == 0) total[blockIdx.x] = before;
 }
 
-// SCANNED: counts and total are the scan's; else counts are plain and tiles <= kFewTiles
+// SCANNED: counts[bin][tile] and total are the scan's; else counts[tile][bin] are plain and few
 template <bool SCANNED>
 __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_place(const int32_t* __restrict__ ids, uint64_t n, uint32_t experts,
                                                                       uint32_t bits, uint32_t tiles, const uint32_t* __restrict__ counts,
                                                                       const uint32_t* __restrict__ total, int32_t* __restrict__ offsets,
                                                                       int32_t* __restrict__ order) {
   __shared__ uint32_t next[kGroupBins + 1];
-  __shared__ uint16_t in_wave[kGroupWaves][kGroupBins];
+  __shared__ __attribute__((aligned(16))) uint16_t in_wave[kGroupBins][kGroupWaves];
   __shared__ uint32_t carry[kGroupWaves];
   __shared__ uint32_t sums[SCANNED ? 1 : kGroupBins + 1];
   const uint32_t bins = experts + 1;
   const uint32_t i0 = 2 * threadIdx.x, i1 = i0 + 1;
   if constexpr (!SCANNED) {
-    const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t bin = threadIdx.x >> 6; bin < bins; bin += kGroupWaves) {
-      const uint32_t c = lane < tiles ? counts[(uint64_t)bin * tiles + lane] : 0;
-      uint32_t all = c, before = lane < blockIdx.x ? c : 0;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        all += (uint32_t)__shfl_xor((int)all, d, 64);
-        before += (uint32_t)__shfl_xor((int)before, d, 64);
+    // counts[tile][bin]: as many threads per bin as there are bins to go round, each adds up its share of the tiles
+    for (uint32_t b = threadIdx.x; b < bins; b += kGroupThreads) sums[b] = next[b] = 0;
+    __syncthreads();
+    uint32_t width = 1;
+    while (width < bins && width < kGroupThreads) width <<= 1;
+    const uint32_t parts = kGroupThreads / width, part = threadIdx.x / width;
+    for (uint32_t bin = threadIdx.x % width; bin < bins; bin += width) {
+      uint32_t all = 0, before = 0;
+#pragma unroll 8
+      for (uint32_t t = part; t < tiles; t += parts) {
+        const uint32_t c = counts[(uint64_t)t * bins + bin];
+        all += c;
+        before += t < blockIdx.x ? c : 0u;
       }
-      if (lane == 0) {
-        sums[bin] = all;
-        next[bin] = before;
-      }
+      if (all) atomicAdd(&sums[bin], all);
+      if (before) atomicAdd(&next[bin], before);
     }
     __syncthreads();
   }
@@ -185,7 +194,7 @@ __global__ __launch_bounds__(kGroupThreads) void hps_group_rows_place(const int3
     if (blockIdx.x == 0) offsets[i1] = (int32_t)b;
   }
   __syncthreads();
-  place_tile(ids, n, (uint64_t)blockIdx.x * kGroupTile, experts, bits, next, in_wave, order);
+  place_tile<false>(ids, n, (uint64_t)blockIdx.x * kGroupTile, experts, bits, next, in_wave, order);
 }
 
 uint64_t GroupRowsWorkspaceBytes(uint64_t n, uint32_t experts) {
@@ -205,8 +214,10 @@ hipError_t LaunchGroupRows(const int32_t* d_ids, uint64_t n, uint32_t experts, i
   const uint32_t tiles = (uint32_t)((n + kGroupTile - 1) / kGroupTile);
   uint32_t* counts = (uint32_t*)d_workspace;
   uint32_t* total = counts + (uint64_t)(experts + 1) * tiles;
-  hps_group_rows_count<<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, tiles, counts);
-  if (tiles <= kFewTiles) {
+  const uint64_t bins = experts + 1;
+  const bool few = tiles <= kFewTiles && tiles * bins <= kFewCounts;
+  hps_group_rows_count<<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, few ? 1 : tiles, few ? bins : 1, counts);
+  if (few) {
     hps_group_rows_place<false><<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
     return hipGetLastError();
   }

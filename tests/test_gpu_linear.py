@@ -187,7 +187,7 @@ def _group_ref(ids, e):
 
 
 @pytest.mark.parametrize("n,e", [(0, 1), (0, 1024), (1, 1), (63, 2), (64, 3), (65, 7), (1000, 1), (1024, 16), (1025, 64), (5000, 1000), (8192, 1024), (8193, 5),
-                                 (9000, 1024), (65536, 16), (65536, 1024), (65537, 700), (70001, 1024), (100000, 1), (3_000_000, 37)])
+                                 (9000, 1024), (4096, 673), (4097, 673), (12288, 1023), (12289, 1023), (49152, 255), (49153, 255), (65536, 16), (65536, 1024), (65537, 700), (70001, 1024), (100000, 1), (3_000_000, 37)])
 def test_group_rows_is_a_stable_sort(n, e):
     import torch
     from hugectr_backend_amd.dense import group_rows
