@@ -164,6 +164,7 @@ __global__ __launch_bounds__(kThreads) void hps_probe_tile_kernel(const CallDesc
 
   if (tid < 4) sh_cnt[tid] = 0;
   if (kDedup) {
+#pragma unroll
     for (uint32_t e = tid; e < (uint32_t)kTileSet; e += kThreads) sh_set[e] = 0xFFFFFFFFu;
   }
   int64_t k[kPerThread];
