@@ -131,13 +131,14 @@ class ExpertLayers:
 
     def forward(self, x, offsets, rows_in=None, rows_out=None, mul=None, residual=None, out=None, out_dtype=None):
         """x: CUDA `dtype` [x_rows, in_dim] (rows may be apart).  offsets: CUDA int32 [num_experts + 1]; expert e has the positions
-        [offsets[e], offsets[e+1]) (clamped to the positions there are, read as their running maximum).  rows_in / rows_out: None or
+        [offsets[e], offsets[e+1]) (clamped to the positions there are, read as their running maximum); None with one expert: all of
+        them.  rows_in / rows_out: None or
         CUDA int32, one entry per position: the row of x it reads (outside x: zeros) and the row of out, mul and residual it has
         (outside out: not written; a row named twice holds, element by element, the result of either).
         Without them position p is row p.  group_rows() makes offsets and such an index from expert numbers.
         out: [rows, out_dim] of `dtype` or fp32; rows of no run stay as they were.  Without `out` a new tensor of `out_dtype` is
         returned, one row per position, and rows of no run are zero (rows_out then names every row once).
-        mul, residual: None or `dtype`, rows like out's; either may be `out` itself.
+        mul, residual: None or `dtype`, rows like out's; either may be `out` itself (rows_out then names no row twice).
         Runs on torch's current stream; may be captured; calls may overlap."""
         p = rows_in if rows_in is not None else rows_out
         rows = x.shape[0] if p is None else p.shape[0]
@@ -161,8 +162,7 @@ class ExpertLayers:
         if residual is not None:
             a.residual, a.residual_stride = self._beside(residual, out, "residual")
         a.rows = rows
-        if offsets is not None:
-            a.offsets, a.rows_in, a.rows_out = offsets, rows_in, rows_out
+        a.offsets, a.rows_in, a.rows_out = offsets, rows_in, rows_out
         rc = hps.LIB.hps_linear_forward(self._h, C.addressof(a), current_stream(self.device))
         if rc:
             hps._check(rc)

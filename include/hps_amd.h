@@ -460,7 +460,7 @@ int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dens
  * ties to even; a < 2^-100: scale 0 and codes 0; a NaN or an infinity in the group: scale NaN, so the group reads back as NaN.
  * A slot outside [0, num_rows) is skipped; of a slot that is named several times in one call the last row stays.
  * read: out = fp32(code * scale) rounded to `type`; a slot outside [0, num_rows) reads as default_value.
- * All pointers on `device`, strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
+ * All pointers on `device` and aligned to their elements, strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
  * be captured into a graph.  One write at a time per store; reads beside reads are free. */
 typedef struct hps_qrows {
   void* codes;
@@ -494,7 +494,7 @@ typedef struct hps_linear_args {
   const void* x;              /* the layer's type, [x_rows] rows x_stride apart (strides in elements) */
   uint64_t x_stride, x_rows;
   void* out;                  /* out_type, [out_rows] rows out_stride apart; may be mul or residual itself, else apart from all inputs */
-  uint64_t out_stride, out_rows;
+  uint64_t out_stride, out_rows;   /* (out as its own mul or residual: rows_out names no row twice) */
   int32_t out_type;           /* the layer's type or HPS_TYPE_FP32 */
   int32_t zero_rest;          /* positions of no run: 0 = their output rows stay as they were, 1 = they become zeros */
   const void* mul;            /* null, or the layer's type, rows like out's */

@@ -367,3 +367,19 @@ def test_two_streams_through_one_layer():
             got.append(layer.forward(x))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.parametrize("rows", [7, 300, 3000])
+def test_one_expert_without_offsets_takes_its_row_indexes(rows):
+    import torch
+    from hugectr_backend_amd.dense import ExpertLayers
+    x, w, b = _operands(torch, 50, 40, 70, torch.float16, rows)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows)
+    rin = torch.randint(0, 50, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    rout = torch.randperm(rows, generator=g, device="cuda").int()
+    layer = ExpertLayers(w, b, activation="relu")
+    _check(layer.forward(x, None, rows_in=rin), x[rin.long()], w[0], b[0], "relu")
+    got = layer.forward(x, None, rows_in=rin, rows_out=rout)
+    _check(got[rout.long()], x[rin.long()], w[0], b[0], "relu")
+    _check(layer.forward(x, None), x, w[0], b[0], "relu")
