@@ -859,6 +859,8 @@ int hps_qrows_write_device(int device, const hps_qrows_t* store, const void* d_r
     if (n >= (1ull << 31)) return Error(Code::kUnsupported, "quantised rows: more than 2^31 rows per call");
     if (n == 0) return Status::Ok();
     if (!d_rows || !d_slots) return Error(Code::kInvalidArg, "null argument");
+    if ((uintptr_t)d_rows % ElemBytes(t) || (uintptr_t)d_held % ElemBytes(t) || (uintptr_t)d_slots % 8)
+      return Error(Code::kInvalidArg, "quantised rows: rows, held and slots are aligned to their elements");
     if (row_stride < d.dim || (d_held && held_stride < d.dim)) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
     if (d_held && !(d_held == d_rows && held_stride == row_stride)) {
       const uintptr_t r = (uintptr_t)d_rows, h = (uintptr_t)d_held;
@@ -883,6 +885,7 @@ int hps_qrows_read_device(int device, const hps_qrows_t* store, const int64_t* d
     if (n >= (1ull << 31)) return Error(Code::kUnsupported, "quantised rows: more than 2^31 rows per call");
     if (n == 0) return Status::Ok();
     if (!d_slots || !d_out) return Error(Code::kInvalidArg, "null argument");
+    if ((uintptr_t)d_out % ElemBytes(t) || (uintptr_t)d_slots % 8) return Error(Code::kInvalidArg, "quantised rows: out and slots are aligned to their elements");
     if (out_stride < d.dim) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
     DeviceGuard guard;
     HPS_RETURN_IF_ERROR(guard.Enter(device));
@@ -943,6 +946,7 @@ int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t
     if (num_experts == 0 || num_experts > kMaxExperts) return Error(Code::kInvalidArg, "grouping: 1..", kMaxExperts, " experts supported, got ", num_experts);
     if (n >= (1ull << 31)) return Error(Code::kUnsupported, "grouping: more than 2^31 rows per call");
     if (!d_offsets || (n && (!d_ids || !d_order)) || (GroupRowsWorkspaceBytes(n, num_experts) && !d_workspace)) return Error(Code::kInvalidArg, "null argument");
+    if (((uintptr_t)d_ids | (uintptr_t)d_offsets | (uintptr_t)d_order | (uintptr_t)d_workspace) % 4) return Error(Code::kInvalidArg, "grouping: a pointer that is not 4-byte aligned");
     DeviceGuard guard;
     HPS_RETURN_IF_ERROR(guard.Enter(device));
     const hipError_t e = LaunchGroupRows(d_ids, n, num_experts, d_offsets, d_order, d_workspace, (hipStream_t)stream);

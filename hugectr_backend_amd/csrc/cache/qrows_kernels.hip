@@ -30,9 +30,7 @@
 
 namespace hps {
 
-typedef float f4q __attribute__((ext_vector_type(4)));
-typedef uint32_t u2q __attribute__((ext_vector_type(2)));
-typedef uint32_t u4q __attribute__((ext_vector_type(4)));
+typedef uint32_t u2q __attribute__((ext_vector_type(2), aligned(4)));   // (codes are 4-byte aligned)
 
 constexpr int kQThreads = 256;
 constexpr uint64_t kQRowsPerLaunch = 1ull << 24;   // a launch holds at most 2^32 threads; a row takes up to 64

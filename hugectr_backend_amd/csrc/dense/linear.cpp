@@ -113,6 +113,9 @@ Status LinearLayers::Forward(const LinearArgs& a, ElemType out_type, hipStream_t
   if (!a.rows_in && a.x_rows < a.rows) return Error(Code::kInvalidArg, "linear forward: ", a.rows, " rows of an input of ", a.x_rows);
   if (!a.rows_out && a.out_rows < a.rows) return Error(Code::kInvalidArg, "linear forward: ", a.rows, " rows into an output of ", a.out_rows);
   const uint64_t in = ElemBytes(type_), ob = ElemBytes(out_type);
+  if ((uintptr_t)a.x % in || (uintptr_t)a.out % ob || (uintptr_t)a.mul % in || (uintptr_t)a.residual % in || (uintptr_t)a.offsets % 4 ||
+      (uintptr_t)a.rows_in % 4 || (uintptr_t)a.rows_out % 4)
+    return Error(Code::kInvalidArg, "linear forward: a pointer that is not aligned to its elements");
   const Span so(a.out, a.out_rows, a.out_stride, d.N, ob), sx(a.x, a.x_rows, a.x_stride, d.K, in);
   if (so.meets(sx)) return Error(Code::kInvalidArg, "linear forward: the output overlaps the input");
   // in place over mul or residual: every element is read by the thread that writes it

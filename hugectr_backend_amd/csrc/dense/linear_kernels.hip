@@ -162,9 +162,10 @@ __device__ __forceinline__ RowTile find_tile(const LinearDesc& d, const LinearAr
   return {2, 0, (uint32_t)first, min((uint32_t)BM, rows - (uint32_t)first)};
 }
 
-// tiles of every expert's runs and of the rest, at most
+// tiles of the runs that are not empty and of the rest before and behind them, at most
 static uint64_t RowTiles(const LinearDesc& d, const LinearArgs& a, uint32_t BM) {
-  return a.offsets ? a.rows / BM + d.experts + 2 : (a.rows + BM - 1) / BM;
+  if (!a.offsets) return (a.rows + BM - 1) / BM;
+  return a.rows / BM + (d.experts < a.rows ? d.experts : a.rows) + (a.zero_rest ? 2 : 0);
 }
 
 // Workgroups go to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, so that tiles that share rows or weights share its L2

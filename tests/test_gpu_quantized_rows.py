@@ -248,3 +248,24 @@ def test_streams_and_a_replayed_graph():
         want = plain.read(s)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(store.codes, plain.codes) and torch.equal(store.scales, plain.scales), k
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_more_rows_than_one_launch_holds(in_place):
+    """2^24 rows are one launch; the rows at both sides of the border, and slots named at both sides of it."""
+    import torch
+    from hugectr_backend_amd.quantized_rows import QuantizedRows
+    n, R = (1 << 24) + 1000, (1 << 24) - 500
+    store = QuantizedRows(R, 1)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = torch.randn(n, 1, generator=g, device="cuda").abs() + 0.5          # one value a row: code 127, scale x / 127
+    slots = torch.arange(n, device="cuda") % R                             # the first 1,500 slots are named twice
+    scale = (x.double() / 127).float()                                     # (torch divides fp32 by a number as a product with 1 / 127)
+    want = scale[:R].clone()
+    want[:1500] = scale[R:]
+    rows = x.clone()
+    held = store.write(rows, slots, held=rows if in_place else torch.empty_like(x))
+    assert torch.equal(held, 127.0 * scale)
+    assert torch.equal(store.scales, want) and (store.codes[:, 0] == 127).all()
+    assert torch.equal(store.read(slots), 127.0 * want[slots])

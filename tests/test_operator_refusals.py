@@ -55,6 +55,10 @@ def test_write_and_read_arguments():
     assert _write(s, held=P + (1 << 20), held_stride=3) == hps.ERR_INVALID_ARG
     assert _write(s, held=P + 64, held_stride=16) == hps.ERR_INVALID_ARG and "overlaps" in _msg()
     assert _write(s, held=P, held_stride=32) == hps.ERR_INVALID_ARG and "overlaps" in _msg()
+    for kw in (dict(rows=P + 1), dict(rows=P + 2), dict(type=1, rows=P + 1), dict(slots=P + 4), dict(held=P + (1 << 20) + 2, held_stride=16)):
+        assert _write(s, **kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
+    for kw in (dict(out=P + 2), dict(type=2, out=P + 1), dict(slots=P + 4)):
+        assert _read(s, **kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
     assert _write(s, n=1 << 31) == hps.ERR_UNSUPPORTED and _read(s, n=1 << 31) == hps.ERR_UNSUPPORTED
     assert _write(s, rows=None, slots=None, n=0) == 0 and _read(s, slots=None, out=None, n=0) == 0
 
@@ -81,6 +85,8 @@ def test_grouping_arguments():
     assert call(n=1 << 31) == hps.ERR_UNSUPPORTED
     assert call(off=None) == hps.ERR_INVALID_ARG and call(ids=None) == hps.ERR_INVALID_ARG and call(order=None) == hps.ERR_INVALID_ARG
     assert L.hps_group_rows_workspace_bytes(10, 4) == 0 and L.hps_group_rows_workspace_bytes(100000, 4) > 0
+    for kw in (dict(ids=P + 2), dict(off=P + 1), dict(order=P + 2), dict(n=100000, work=P + 2)):
+        assert call(**kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
     assert call(n=100000) == hps.ERR_INVALID_ARG      # needs its workspace
 
 
@@ -139,6 +145,16 @@ def test_refusals_of_a_layer_and_of_the_wrappers():
         lambda: store.read(slots, out=rows, dtype=torch.float16),
         lambda: QuantizedRows(-1, 8), lambda: QuantizedRows(1, 0), lambda: QuantizedRows(1, 8, bits=5), lambda: QuantizedRows(1, 8, group=24),
     ]
+    def odd(**kw):       # at the C boundary: pointers that torch does not make
+        a = hps.LinearArgs(x.data_ptr(), 8, 5, half.data_ptr(), 6, 5, 1, 0)
+        a.rows = 5
+        for name, value in kw.items():
+            setattr(a, name, value)
+        hps._check(L.hps_linear_forward(layer._h, C.addressof(a), None))
+    odd()
+    bad += [lambda: odd(x=x.data_ptr() + 1), lambda: odd(out=half.data_ptr() + 1), lambda: odd(out_type=0, out=big.data_ptr() + 2),
+            lambda: odd(mul=big.data_ptr() + 1, mul_stride=14), lambda: odd(residual=big.data_ptr() + 1, residual_stride=14),
+            lambda: odd(rows_in=idx.data_ptr() + 2), lambda: odd(rows_out=idx.data_ptr() + 1), lambda: odd(offsets=off.data_ptr() + 2)]
     for k, f in enumerate(bad):
         with pytest.raises(hps.HpsError) as e:
             f()
