@@ -414,7 +414,8 @@ bool Aligned(const void* p, uint64_t stride, uint32_t dim, uint32_t V, uint32_t 
 
 // kStamp costs one launch more than kClaim (5 us in all) and saves 25 us a million rows
 constexpr uint64_t kStampRows = 1ull << 18;
-constexpr uint32_t kListBlocks = 256;
+// the last pass: 1.7 M rows, 17,000 of them listed, 256 / 512 / 1,024 / 2,048 blocks 259.7 / 255.3 / 253.3 / 252.5 us, none listed 246.8 - 247.1
+constexpr uint32_t kListBlocks = 1024;
 
 template <typename T, int BITS, bool VEC, int NCH>
 hipError_t WriteKept(const QRowsDesc& s, const T* rows, uint64_t row_stride, const int64_t* slots, uint64_t n, T* held, uint64_t held_stride,
