@@ -79,6 +79,7 @@ class QuantizedRows:
                                     self.bits, self.group)
         self._desc_p = C.addressof(self._desc)
         self._slot_type = torch.int64
+        self._like = {}        # an empty tensor of every type read so far: new_empty of the same type is 0.5 us of a call less
 
     def _slots(self, slots) -> int:
         if slots.dtype != self._slot_type or slots.get_device() != self.device or slots.dim() != 1 or not slots.is_contiguous():
@@ -111,12 +112,17 @@ class QuantizedRows:
         import torch
         n = self._slots(slots)
         if out is None:
-            out = slots.new_empty((n, self.dim), dtype=dtype or torch.float32)
-        elif dtype is not None and out.dtype != dtype:
-            raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
-        stride = row_stride(out, self.dim, "out", self.device)
-        if out.shape[0] != n:
-            raise _invalid(f"out: {n} rows expected, got {out.shape[0]}")
+            like = self._like.get(dtype)
+            if like is None:
+                elem_type(dtype or torch.float32)
+                like = self._like[dtype] = torch.empty(0, dtype=dtype or torch.float32, device=self.codes.device)
+            out, stride = like.new_empty((n, self.dim)), self.dim
+        else:
+            if dtype is not None and out.dtype != dtype:
+                raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
+            stride = row_stride(out, self.dim, "out", self.device)
+            if out.shape[0] != n:
+                raise _invalid(f"out: {n} rows expected, got {out.shape[0]}")
         hps._check(hps.LIB.hps_qrows_read_device(self.device, self._desc_p, slots.data_ptr(), n, default_value, out.data_ptr(),
                                                  elem_type(out.dtype), stride, current_stream(self.device)))
         return out
