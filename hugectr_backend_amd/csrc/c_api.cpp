@@ -20,6 +20,7 @@
 #include "cache/qrows.h"
 #include "cache/shard_session.h"
 #include "common/device_guard.h"
+#include "common/span.h"
 #include "dense/dense.h"
 #include "dense/linear.h"
 
@@ -842,6 +843,10 @@ Status QRowsStore(const hps_qrows_t* store, bool write, QRowsDesc* d) {
   d->row_bytes = QRowsRowBytes(store->dim, store->bits);
   return Status::Ok();
 }
+bool OverStore(const QRowsDesc& d, const Span& s, bool workspace) {
+  return s.meets(Span(d.codes, d.num_rows, d.row_bytes, d.row_bytes, 1)) || s.meets(Span(d.scales, d.num_rows, d.groups, d.groups, 4)) ||
+         (workspace && s.meets(Span(d.claim, 1, 0, QRowsWorkspaceBytes(d.num_rows), 1)));
+}
 Status ElemTypeOf(int type, ElemType* t) {
   if (type < HPS_TYPE_FP32 || type > HPS_TYPE_BF16) return Error(Code::kInvalidArg, "unknown element type ", type);
   *t = (ElemType)type;
@@ -862,11 +867,11 @@ int hps_qrows_write_device(int device, const hps_qrows_t* store, const void* d_r
     if ((uintptr_t)d_rows % ElemBytes(t) || (uintptr_t)d_held % ElemBytes(t) || (uintptr_t)d_slots % 8)
       return Error(Code::kInvalidArg, "quantised rows: rows, held and slots are aligned to their elements");
     if (row_stride < d.dim || (d_held && held_stride < d.dim)) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
-    if (d_held && !(d_held == d_rows && held_stride == row_stride)) {
-      const uintptr_t r = (uintptr_t)d_rows, h = (uintptr_t)d_held;
-      const uint64_t rb = ((n - 1) * row_stride + d.dim) * ElemBytes(t), hb = ((n - 1) * held_stride + d.dim) * ElemBytes(t);
-      if (r < h + hb && h < r + rb) return Error(Code::kInvalidArg, "quantised rows: held overlaps the rows without being the same rows");
-    }
+    const Span rows(d_rows, n, row_stride, d.dim, ElemBytes(t)), held(d_held, n, held_stride, d.dim, ElemBytes(t)), at(d_slots, 1, 0, n, 8);
+    if (held.meets(rows) && !(d_held == d_rows && held_stride == row_stride))
+      return Error(Code::kInvalidArg, "quantised rows: held overlaps the rows without being the same rows");
+    if (held.meets(at) || OverStore(d, rows, true) || OverStore(d, held, true) || OverStore(d, at, true))
+      return Error(Code::kInvalidArg, "quantised rows: held overlaps the slots, or an operand the store");
     DeviceGuard guard;
     HPS_RETURN_IF_ERROR(guard.Enter(device));
     const hipError_t e = LaunchQRowsWrite(d, d_rows, t, row_stride, d_slots, n, d_held, held_stride, (hipStream_t)stream);
@@ -887,6 +892,8 @@ int hps_qrows_read_device(int device, const hps_qrows_t* store, const int64_t* d
     if (!d_slots || !d_out) return Error(Code::kInvalidArg, "null argument");
     if ((uintptr_t)d_out % ElemBytes(t) || (uintptr_t)d_slots % 8) return Error(Code::kInvalidArg, "quantised rows: out and slots are aligned to their elements");
     if (out_stride < d.dim) return Error(Code::kInvalidArg, "quantised rows: rows are closer together than they are wide");
+    const Span out(d_out, n, out_stride, d.dim, ElemBytes(t));
+    if (out.meets(Span(d_slots, 1, 0, n, 8)) || OverStore(d, out, false)) return Error(Code::kInvalidArg, "quantised rows: out overlaps the slots or the store");
     DeviceGuard guard;
     HPS_RETURN_IF_ERROR(guard.Enter(device));
     const hipError_t e = LaunchQRowsRead(d, d_slots, n, default_value, d_out, t, out_stride, (hipStream_t)stream);
@@ -947,6 +954,10 @@ int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t
     if (n >= (1ull << 31)) return Error(Code::kUnsupported, "grouping: more than 2^31 rows per call");
     if (!d_offsets || (n && (!d_ids || !d_order)) || (GroupRowsWorkspaceBytes(n, num_experts) && !d_workspace)) return Error(Code::kInvalidArg, "null argument");
     if (((uintptr_t)d_ids | (uintptr_t)d_offsets | (uintptr_t)d_order | (uintptr_t)d_workspace) % 4) return Error(Code::kInvalidArg, "grouping: a pointer that is not 4-byte aligned");
+    const Span ids(d_ids, 1, 0, n, 4), offsets(d_offsets, 1, 0, (uint64_t)num_experts + 1, 4), order(d_order, 1, 0, n, 4),
+        work(d_workspace, 1, 0, GroupRowsWorkspaceBytes(n, num_experts), 1);
+    if (ids.meets(offsets) || ids.meets(order) || offsets.meets(order) || work.meets(ids) || work.meets(offsets) || work.meets(order))
+      return Error(Code::kInvalidArg, "grouping: ids, offsets, order and workspace overlap");
     DeviceGuard guard;
     HPS_RETURN_IF_ERROR(guard.Enter(device));
     const hipError_t e = LaunchGroupRows(d_ids, n, num_experts, d_offsets, d_order, d_workspace, (hipStream_t)stream);

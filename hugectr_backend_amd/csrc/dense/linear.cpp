@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include "../common/device_guard.h"
+#include "../common/span.h"
 
 namespace hps {
 
@@ -27,17 +28,6 @@ struct DeviceBuffer {
     p = nullptr;
     return q;
   }
-};
-
-// [first byte, last byte] of a [rows][stride] block of `width` elements
-struct Span {
-  uintptr_t lo = 0, hi = 0;
-  Span(const void* p, uint64_t rows, uint64_t stride, uint64_t width, uint64_t bytes) {
-    if (!p || rows == 0 || width == 0) return;
-    lo = (uintptr_t)p;
-    hi = lo + ((rows - 1) * stride + width) * bytes;
-  }
-  bool meets(const Span& o) const { return hi != 0 && o.hi != 0 && lo < o.hi && o.lo < hi; }
 };
 
 }  // namespace
@@ -118,6 +108,8 @@ Status LinearLayers::Forward(const LinearArgs& a, ElemType out_type, hipStream_t
     return Error(Code::kInvalidArg, "linear forward: a pointer that is not aligned to its elements");
   const Span so(a.out, a.out_rows, a.out_stride, d.N, ob), sx(a.x, a.x_rows, a.x_stride, d.K, in);
   if (so.meets(sx)) return Error(Code::kInvalidArg, "linear forward: the output overlaps the input");
+  if (so.meets(Span(a.offsets, 1, 0, (uint64_t)d.experts + 1, 4)) || so.meets(Span(a.rows_in, 1, 0, a.rows, 4)) || so.meets(Span(a.rows_out, 1, 0, a.rows, 4)))
+    return Error(Code::kInvalidArg, "linear forward: the output overlaps offsets or row indexes");
   // in place over mul or residual: every element is read by the thread that writes it
   auto apart = [&](const void* p, uint64_t stride) {
     const bool same = p == a.out && stride == a.out_stride && ob == in;

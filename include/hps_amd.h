@@ -460,7 +460,7 @@ int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dens
  * ties to even; a < 2^-100: scale 0 and codes 0; a NaN or an infinity in the group: scale NaN, so the group reads back as NaN.
  * A slot outside [0, num_rows) is skipped; of a slot that is named several times in one call the last row stays.
  * read: out = fp32(code * scale) rounded to `type`; a slot outside [0, num_rows) reads as default_value.
- * All pointers on `device` and aligned to their elements, strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
+ * All pointers on `device`, aligned to their elements and apart from each other (but for d_held), strides in elements, enqueued on `stream` (a hipStream_t of that device), not synchronised; both may
  * be captured into a graph.  One write at a time per store; reads beside reads are free. */
 typedef struct hps_qrows {
   void* codes;
@@ -517,7 +517,7 @@ void hps_linear_destroy(hps_linear_t* layer);
 int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void* stream);
 /* The runs an expert layer needs: a stable sort of the positions 0 .. n-1 by d_ids[position].  d_offsets[num_experts + 1], d_order[n]:
  * the positions of expert e are d_order[offsets[e] .. offsets[e+1]); ids outside [0, num_experts) come behind the last run.
- * n < 2^31, num_experts <= 1024; d_workspace: hps_group_rows_workspace_bytes (may be null where that is 0), one call at a time. */
+ * All apart from each other.  n < 2^31, num_experts <= 1024; d_workspace: hps_group_rows_workspace_bytes (may be null where that is 0), one call at a time. */
 uint64_t hps_group_rows_workspace_bytes(uint64_t n, uint32_t num_experts);
 int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t num_experts, int32_t* d_offsets, int32_t* d_order,
                           void* d_workspace, void* stream);

@@ -8,21 +8,22 @@ from hugectr_backend_amd import hps
 
 L = hps.LIB
 P = 0x10000           # some address; no check follows it
+CODES, SCALES, WORK, SLOTS = (P + (k << 24) for k in range(1, 5))
 
 
 def _store(**kw):
-    return hps.QRowsStore(**{**dict(codes=P, scales=P, workspace=P, num_rows=100, dim=16, bits=8, group=0), **kw})
+    return hps.QRowsStore(**{**dict(codes=CODES, scales=SCALES, workspace=WORK, num_rows=100, dim=16, bits=8, group=0), **kw})
 
 
 def _msg():
     return L.hps_last_error().decode()
 
 
-def _write(store, rows=P, type=0, stride=16, slots=P, n=4, held=None, held_stride=0):
+def _write(store, rows=P, type=0, stride=16, slots=SLOTS, n=4, held=None, held_stride=0):
     return L.hps_qrows_write_device(0, C.addressof(store) if store is not None else None, rows, type, stride, slots, n, held, held_stride, None)
 
 
-def _read(store, slots=P, n=4, out=P, type=0, stride=16):
+def _read(store, slots=SLOTS, n=4, out=P, type=0, stride=16):
     return L.hps_qrows_read_device(0, C.addressof(store) if store is not None else None, slots, n, 0.0, out, type, stride, None)
 
 
@@ -35,7 +36,7 @@ def test_row_geometry():
 @pytest.mark.parametrize("kw,word", [
     (dict(dim=0), "values per row"), (dict(dim=16385), "values per row"), (dict(bits=2), "8 or 4 bits"), (dict(bits=0), "8 or 4 bits"),
     (dict(group=17), "a scale per row"), (dict(group=512), "a scale per row"), (dict(codes=None), "null store"), (dict(scales=None), "null store"),
-    (dict(codes=P + 2), "aligned"), (dict(scales=P + 1), "aligned"),
+    (dict(codes=CODES + 2), "aligned"), (dict(scales=SCALES + 1), "aligned"),
 ])
 def test_stores_that_cannot_be(kw, word):
     for call in (_write, _read):
@@ -55,10 +56,15 @@ def test_write_and_read_arguments():
     assert _write(s, held=P + (1 << 20), held_stride=3) == hps.ERR_INVALID_ARG
     assert _write(s, held=P + 64, held_stride=16) == hps.ERR_INVALID_ARG and "overlaps" in _msg()
     assert _write(s, held=P, held_stride=32) == hps.ERR_INVALID_ARG and "overlaps" in _msg()
-    for kw in (dict(rows=P + 1), dict(rows=P + 2), dict(type=1, rows=P + 1), dict(slots=P + 4), dict(held=P + (1 << 20) + 2, held_stride=16)):
+    for kw in (dict(rows=P + 1), dict(rows=P + 2), dict(type=1, rows=P + 1), dict(slots=SLOTS + 4), dict(held=P + (1 << 20) + 2, held_stride=16)):
         assert _write(s, **kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
-    for kw in (dict(out=P + 2), dict(type=2, out=P + 1), dict(slots=P + 4)):
+    for kw in (dict(out=P + 2), dict(type=2, out=P + 1), dict(slots=SLOTS + 4)):
         assert _read(s, **kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
+    for kw in (dict(held=SLOTS - 64, held_stride=16), dict(rows=CODES + 64), dict(rows=SCALES - 4), dict(slots=WORK + 8),
+               dict(held=CODES + 1596, held_stride=16), dict(rows=WORK + (2 * 100 + 65535) * 4)):
+        assert _write(s, **kw) == hps.ERR_INVALID_ARG and "overlap" in _msg(), kw
+    for kw in (dict(out=SLOTS + 28), dict(out=CODES - 252), dict(out=SCALES + 396), dict(out=P, n=1 << 30)):
+        assert _read(s, **kw) == hps.ERR_INVALID_ARG and "overlap" in _msg(), kw
     assert _write(s, n=1 << 31) == hps.ERR_UNSUPPORTED and _read(s, n=1 << 31) == hps.ERR_UNSUPPORTED
     assert _write(s, rows=None, slots=None, n=0) == 0 and _read(s, slots=None, out=None, n=0) == 0
 
@@ -80,13 +86,15 @@ def test_layers_that_cannot_be():
 
 
 def test_grouping_arguments():
-    call = lambda n=10, e=4, ids=P, off=P, order=P, work=None: L.hps_group_rows_device(0, ids, n, e, off, order, work, None)  # noqa: E731
+    call = lambda n=10, e=4, ids=P, off=CODES, order=SCALES, work=None: L.hps_group_rows_device(0, ids, n, e, off, order, work, None)  # noqa: E731
     assert call(e=0) == hps.ERR_INVALID_ARG and call(e=1025) == hps.ERR_INVALID_ARG and "1..1024" in _msg()
     assert call(n=1 << 31) == hps.ERR_UNSUPPORTED
     assert call(off=None) == hps.ERR_INVALID_ARG and call(ids=None) == hps.ERR_INVALID_ARG and call(order=None) == hps.ERR_INVALID_ARG
     assert L.hps_group_rows_workspace_bytes(10, 4) == 0 and L.hps_group_rows_workspace_bytes(100000, 4) > 0
-    for kw in (dict(ids=P + 2), dict(off=P + 1), dict(order=P + 2), dict(n=100000, work=P + 2)):
+    for kw in (dict(ids=P + 2), dict(off=CODES + 1), dict(order=SCALES + 2), dict(n=100000, work=WORK + 2)):
         assert call(**kw) == hps.ERR_INVALID_ARG and "aligned" in _msg(), kw
+    for kw in (dict(order=P), dict(order=P + 36), dict(off=P - 16), dict(off=SCALES + 36), dict(n=100000, work=CODES), dict(n=100000, work=SCALES + 399996)):
+        assert call(**kw) == hps.ERR_INVALID_ARG and "overlap" in _msg(), kw
     assert call(n=100000) == hps.ERR_INVALID_ARG      # needs its workspace
 
 
@@ -99,7 +107,7 @@ def test_without_a_device_every_call_says_so():
     s = _store()
     assert _write(s) == hps.ERR_UNAVAILABLE and _read(s) == hps.ERR_UNAVAILABLE and "no CPU fallback" in _msg()
     assert _create() == hps.ERR_UNAVAILABLE
-    assert L.hps_group_rows_device(0, P, 10, 4, P, P, None, None) == hps.ERR_UNAVAILABLE
+    assert L.hps_group_rows_device(0, P, 10, 4, CODES, SCALES, None, None) == hps.ERR_UNAVAILABLE
     for make in (lambda: QuantizedRows(4, 4), lambda: LinearLayer(torch.zeros(4, 4))):
         with pytest.raises(hps.HpsError) as e:
             make()
@@ -154,10 +162,15 @@ def test_refusals_of_a_layer_and_of_the_wrappers():
     odd()
     bad += [lambda: odd(x=x.data_ptr() + 1), lambda: odd(out=half.data_ptr() + 1), lambda: odd(out_type=0, out=big.data_ptr() + 2),
             lambda: odd(mul=big.data_ptr() + 1, mul_stride=14), lambda: odd(residual=big.data_ptr() + 1, residual_stride=14),
+            lambda: odd(rows_in=half.data_ptr() + 56), lambda: odd(rows_out=half.data_ptr()), lambda: odd(offsets=half.data_ptr() - 4),
             lambda: odd(rows_in=idx.data_ptr() + 2), lambda: odd(rows_out=idx.data_ptr() + 1), lambda: odd(offsets=off.data_ptr() + 2)]
     for k, f in enumerate(bad):
         with pytest.raises(hps.HpsError) as e:
             f()
         assert e.value.code == hps.ERR_INVALID_ARG, (k, e.value)
+    for call in (lambda: L.hps_group_rows_device(99, idx.data_ptr(), 5, 3, off.data_ptr(), slots.data_ptr(), None, None),
+                 lambda: L.hps_qrows_read_device(99, store._desc_p, slots.data_ptr(), 5, 0.0, rows.data_ptr(), 0, 8, None),
+                 lambda: L.hps_qrows_write_device(-1, store._desc_p, rows.data_ptr(), 0, 8, slots.data_ptr(), 5, None, 0, None)):
+        assert call() == hps.ERR_INVALID_ARG and "not visible" in _msg()
     torch.cuda.synchronize()
     assert layer.forward(x[:0]).shape == (0, 6) and experts.forward(xb[:0], off).shape == (0, 6)
