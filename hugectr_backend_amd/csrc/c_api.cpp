@@ -936,11 +936,11 @@ int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void*
     a.mul_stride = args->mul_stride;
     a.residual = args->residual;
     a.residual_stride = args->residual_stride;
-    a.rows = args->rows;
+    a.rows = args->rows < (1ull << 31) ? (uint32_t)args->rows : 1u << 31;   // (refused)
     a.offsets = args->offsets;
     a.rows_in = args->rows_in;
     a.rows_out = args->rows_out;
-    a.zero_rest = args->zero_rest;
+    a.zero_rest = args->zero_rest != 0;
     return layer->l->Forward(a, t, (hipStream_t)stream);
   });
 }

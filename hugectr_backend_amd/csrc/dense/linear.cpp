@@ -93,7 +93,7 @@ Status LinearLayers::Forward(const LinearArgs& a, ElemType out_type, hipStream_t
   const LinearDesc& d = d_;
   if (out_type != type_ && out_type != ElemType::kF32)
     return Error(Code::kInvalidArg, "linear forward: the output has the layer's type or fp32, got type ", (int)out_type);
-  if (a.rows >= (1ull << 31)) return Error(Code::kUnsupported, "linear forward: more than 2^31 rows per call");
+  if (a.rows >= (1u << 31)) return Error(Code::kUnsupported, "linear forward: more than 2^31 rows per call");
   if (a.rows == 0) return Status::Ok();
   if (!a.x || !a.out) return Error(Code::kInvalidArg, "linear forward: null device pointer");
   if (d.experts > 1 && !a.offsets) return Error(Code::kInvalidArg, "linear forward: ", d.experts, " experts need the offsets of their runs");

@@ -128,7 +128,7 @@ __device__ __forceinline__ uint32_t over_lanes(uint32_t v, Op op) {
 
 template <int BM>
 __device__ __forceinline__ RowTile find_tile(const LinearDesc& d, const LinearArgs& a, uint32_t tile, int lane) {
-  const uint32_t rows = (uint32_t)a.rows;
+  const uint32_t rows = a.rows;
   if (!a.offsets) {
     const uint32_t first = tile * BM;
     if (first >= rows) return {0, 0, 0, 0};
@@ -745,7 +745,7 @@ hipError_t LaunchLinearPack(const void* d_w, ElemType from, uint32_t experts, ui
 
 hipError_t LaunchLinear(const LinearDesc& d, const LinearArgs& args, ElemType type, ElemType out_type, int cu_count, hipStream_t stream) {
   LinearArgs a = args;
-  a.stream_out = a.rows * d.N * ElemBytes(out_type) >= kStreamBytes;
+  a.stream_out = (uint64_t)a.rows * d.N * ElemBytes(out_type) >= kStreamBytes;
   if (type == ElemType::kF16)
     return out_type == ElemType::kF32 ? LaunchTyped<_Float16, float>(d, a, cu_count, stream)
                                       : LaunchTyped<_Float16, _Float16>(d, a, cu_count, stream);

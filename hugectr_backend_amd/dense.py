@@ -6,11 +6,14 @@ csrc/dense/; torch is used for device buffers only.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
 from . import hps
 from .quantized_rows import _invalid, current_stream, elem_type, row_stride
+
+_pack_args = struct.Struct("QQQQQQiiQQQQQQQQ").pack       # an hps.LinearArgs, 0.4 us sooner than field by field
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
@@ -114,6 +117,8 @@ class ExpertLayers:
                 raise _invalid(f"biases: [{w.shape[0]}, {w.shape[2]}] expected, got {tuple(b.shape)}")
         self.num_experts, self.in_dim, self.out_dim = (int(v) for v in w.shape)
         self.dtype, self.activation, self.device = dtype, activation, int(device)
+        self._index_type, self._stream = torch.int32, current_stream()
+        self._like = {t: torch.empty(0, dtype=t, device=dev) for t in (dtype, torch.float32)}   # new_empty of the same type: 0.5 us less
         h = C.c_void_p()
         hps._check(hps.LIB.hps_linear_create(self.device, self.num_experts, self.in_dim, self.out_dim, elem_type(dtype),
                                              ACTIVATIONS[activation], w.data_ptr(), elem_type(w.dtype), b.data_ptr() if b is not None else None,
@@ -121,10 +126,7 @@ class ExpertLayers:
         self._h = h
 
     def _index(self, t, n, name):
-        if t is None:
-            return None
-        import torch
-        if t.dtype != torch.int32 or t.get_device() != self.device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        if t.dtype != self._index_type or t.get_device() != self.device or t.shape != (n,) or not t.is_contiguous():
             raise _invalid(f"{name}: a contiguous vector of {n} int32 on cuda:{self.device} expected, got {t.dtype} {tuple(t.shape)} on "
                            f"{t.device}")
         return t.data_ptr()
@@ -142,28 +144,30 @@ class ExpertLayers:
         Runs on torch's current stream; may be captured; calls may overlap."""
         p = rows_in if rows_in is not None else rows_out
         rows = x.shape[0] if p is None else p.shape[0]
-        return self._run(x, rows, self._index(offsets, self.num_experts + 1, "offsets"), self._index(rows_in, rows, "rows_in"),
-                         self._index(rows_out, rows, "rows_out"), mul, residual, out, out_dtype)
+        o = self._index(offsets, self.num_experts + 1, "offsets") if offsets is not None else 0
+        i = self._index(rows_in, rows, "rows_in") if rows_in is not None else 0
+        j = i if rows_out is rows_in else self._index(rows_out, rows, "rows_out") if rows_out is not None else 0
+        return self._run(x, rows, o, i, j, mul, residual, out, out_dtype)
 
     def _run(self, x, rows, offsets, rows_in, rows_out, mul, residual, out, out_dtype):
         if x.dtype != self.dtype:
             raise _invalid(f"x: {self.dtype} expected, got {x.dtype}")
         stride = row_stride(x, self.in_dim, "x", self.device)
         if out is None:
-            out = x.new_empty((rows, self.out_dim)) if out_dtype is None else x.new_empty((rows, self.out_dim), dtype=out_dtype)
+            like = self._like.get(out_dtype or self.dtype)
+            if like is None:
+                raise _invalid(f"out_dtype: {self.dtype} or torch.float32 expected, got {out_dtype}")
+            out = like.new_empty(rows, self.out_dim)
             zero_rest, out_stride = 1, self.out_dim
         else:
             if out_dtype is not None and out.dtype != out_dtype:
                 raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
             zero_rest, out_stride = 0, row_stride(out, self.out_dim, "out", self.device)
-        a = hps.LinearArgs(x.data_ptr(), stride, x.shape[0], out.data_ptr(), out_stride, out.shape[0], elem_type(out.dtype), zero_rest)
-        if mul is not None:
-            a.mul, a.mul_stride = self._beside(mul, out, "mul")
-        if residual is not None:
-            a.residual, a.residual_stride = self._beside(residual, out, "residual")
-        a.rows = rows
-        a.offsets, a.rows_in, a.rows_out = offsets, rows_in, rows_out
-        rc = hps.LIB.hps_linear_forward(self._h, C.addressof(a), current_stream(self.device))
+        m, ms = (0, 0) if mul is None else self._beside(mul, out, "mul")
+        r, rs = (0, 0) if residual is None else self._beside(residual, out, "residual")
+        a = _pack_args(x.data_ptr(), stride, x.shape[0], out.data_ptr(), out_stride, out.shape[0], elem_type(out.dtype), zero_rest,
+                       m, ms, r, rs, rows, offsets, rows_in, rows_out)
+        rc = hps.LIB.hps_linear_forward(self._h, a, self._stream(self.device))
         if rc:
             hps._check(rc)
         return out
@@ -198,7 +202,7 @@ class LinearLayer(ExpertLayers):
         stream; may be captured; calls may overlap."""
         if out is not None and out.shape[0] != x.shape[0]:
             raise _invalid(f"out: {x.shape[0]} rows expected, got {out.shape[0]}")
-        return self._run(x, x.shape[0], None, None, None, mul, residual, out, out_dtype)
+        return self._run(x, x.shape[0], 0, 0, 0, mul, residual, out, out_dtype)
 
 
 def group_rows(ids, num_experts: int):
@@ -215,6 +219,8 @@ def group_rows(ids, num_experts: int):
     offsets, order = ids.new_empty(num_experts + 1), ids.new_empty(n)
     nbytes = int(hps.LIB.hps_group_rows_workspace_bytes(n, num_experts))
     work = ids.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    hps._check(hps.LIB.hps_group_rows_device(device, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
-                                             work.data_ptr() if work is not None else None, current_stream(device)))
+    rc = hps.LIB.hps_group_rows_device(device, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
+                                       work.data_ptr() if work is not None else None, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        hps._check(rc)
     return offsets, order

@@ -28,27 +28,28 @@ def elem_type(dtype) -> int:
     return t
 
 
-def current_stream(device: int) -> int:
-    """The hipStream_t of torch's current stream (without the Stream object around it: 1 us of a 6-us call)."""
+def current_stream():
+    """device -> hipStream_t of torch's current stream there (without the Stream object around it: 1 us of a 6-us call)."""
     import torch
-    return torch._C._cuda_getCurrentRawStream(device)
+    return torch._C._cuda_getCurrentRawStream
 
 
 def row_stride(t, width: int, name: str, device: int) -> int:
     """Distance of the rows of a 2-D CUDA tensor on `device` whose values lie side by side, `width` of them per row."""
     if t.get_device() != device:
         raise _invalid(f"{name}: a tensor on cuda:{device} expected, got one on {t.device}")
-    shape = t.shape
-    if len(shape) != 2 or shape[1] != width:
-        raise _invalid(f"{name}: rows of {width} values expected, got shape {tuple(shape)}")
-    stride = t.stride()
-    if width > 1 and stride[1] != 1:
-        raise _invalid(f"{name}: the values of a row have to lie side by side")
-    if shape[0] <= 1:
+    if t.dim() != 2 or t.shape[1] != width:
+        raise _invalid(f"{name}: rows of {width} values expected, got shape {tuple(t.shape)}")
+    rows, side = t.stride()
+    if rows == width and side == 1:
         return width
-    if stride[0] < width:
-        raise _invalid(f"{name}: the rows overlap (stride {stride[0]}, {width} values)")
-    return stride[0]
+    if width > 1 and side != 1:
+        raise _invalid(f"{name}: the values of a row have to lie side by side")
+    if t.shape[0] <= 1:
+        return width
+    if rows < width:
+        raise _invalid(f"{name}: the rows overlap (stride {rows}, {width} values)")
+    return rows
 
 
 class QuantizedRows:
@@ -78,7 +79,7 @@ class QuantizedRows:
         self._desc = hps.QRowsStore(self.codes.data_ptr(), self.scales.data_ptr(), self._workspace.data_ptr(), self.num_rows, self.dim,
                                     self.bits, self.group)
         self._desc_p = C.addressof(self._desc)
-        self._slot_type = torch.int64
+        self._slot_type, self._stream = torch.int64, current_stream()
         self._like = {}        # an empty tensor of every type read so far: new_empty of the same type is 0.5 us of a call less
 
     def _slots(self, slots) -> int:
@@ -102,27 +103,31 @@ class QuantizedRows:
             if held.dtype != rows.dtype or held.shape[0] != n:
                 raise _invalid(f"held: {n} rows of {rows.dtype} expected, got {held.shape[0]} of {held.dtype}")
             hp = held.data_ptr()
-        hps._check(hps.LIB.hps_qrows_write_device(self.device, self._desc_p, rows.data_ptr(), elem_type(rows.dtype), stride,
-                                                  slots.data_ptr(), n, hp, hs, current_stream(self.device)))
+        rc = hps.LIB.hps_qrows_write_device(self.device, self._desc_p, rows.data_ptr(), elem_type(rows.dtype), stride, slots.data_ptr(), n, hp,
+                                            hs, self._stream(self.device))
+        if rc:
+            hps._check(rc)
         return held
 
     def read(self, slots, out=None, dtype=None, default_value: float = 0.0):
         """The rows at `slots` (CUDA int64 [n]) as fp32 (or `dtype`: fp16, bf16) [n, dim]; a slot outside [0, num_rows) reads as
         `default_value`.  Runs on torch's current stream; may be captured."""
-        import torch
         n = self._slots(slots)
         if out is None:
             like = self._like.get(dtype)
             if like is None:
+                import torch
                 elem_type(dtype or torch.float32)
                 like = self._like[dtype] = torch.empty(0, dtype=dtype or torch.float32, device=self.codes.device)
-            out, stride = like.new_empty((n, self.dim)), self.dim
+            out, stride = like.new_empty(n, self.dim), self.dim
         else:
             if dtype is not None and out.dtype != dtype:
                 raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
             stride = row_stride(out, self.dim, "out", self.device)
             if out.shape[0] != n:
                 raise _invalid(f"out: {n} rows expected, got {out.shape[0]}")
-        hps._check(hps.LIB.hps_qrows_read_device(self.device, self._desc_p, slots.data_ptr(), n, default_value, out.data_ptr(),
-                                                 elem_type(out.dtype), stride, current_stream(self.device)))
+        rc = hps.LIB.hps_qrows_read_device(self.device, self._desc_p, slots.data_ptr(), n, default_value, out.data_ptr(),
+                                           elem_type(out.dtype), stride, self._stream(self.device))
+        if rc:
+            hps._check(rc)
         return out

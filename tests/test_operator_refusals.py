@@ -174,3 +174,12 @@ def test_refusals_of_a_layer_and_of_the_wrappers():
         assert call() == hps.ERR_INVALID_ARG and "not visible" in _msg()
     torch.cuda.synchronize()
     assert layer.forward(x[:0]).shape == (0, 6) and experts.forward(xb[:0], off).shape == (0, 6)
+
+
+def test_the_packed_arguments_are_the_struct():
+    from hugectr_backend_amd import dense
+    names = ["x", "x_stride", "x_rows", "out", "out_stride", "out_rows", "out_type", "zero_rest", "mul", "mul_stride", "residual", "residual_stride",
+             "rows", "offsets", "rows_in", "rows_out"]
+    assert names == [n for n, _ in hps.LinearArgs._fields_]
+    a = hps.LinearArgs.from_buffer_copy(dense._pack_args(*range(1, 17)))
+    assert [getattr(a, n) for n in names] == list(range(1, 17)) and C.sizeof(a) == len(dense._pack_args(*range(16)))
