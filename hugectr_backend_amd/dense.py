@@ -218,7 +218,7 @@ def group_rows(ids, num_experts: int):
     n = ids.shape[0]
     offsets, order = ids.new_empty(num_experts + 1), ids.new_empty(n)
     nbytes = int(hps.LIB.hps_group_rows_workspace_bytes(n, num_experts))
-    work = ids.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    work = ids.new_empty((nbytes + 3) // 4) if nbytes else None
     rc = hps.LIB.hps_group_rows_device(device, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
                                        work.data_ptr() if work is not None else None, torch._C._cuda_getCurrentRawStream(device))
     if rc:
