@@ -827,7 +827,8 @@ Status QRowsStore(const hps_qrows_t* store, bool write, QRowsDesc* d) {
   const uint32_t g = store->group;
   if (g != 0 && g != 16 && g != 32 && g != 64 && g != 128 && g != 256)
     return Error(Code::kInvalidArg, "quantised rows: a scale per row (0) or per 16, 32, 64, 128 or 256 values, got ", g);
-  if (store->num_rows && (!store->codes || !store->scales || (write && !store->workspace))) return Error(Code::kInvalidArg, "quantised rows: null store pointer");
+  if (store->num_rows && (!store->codes || !store->scales)) return Error(Code::kInvalidArg, "quantised rows: null store pointer");
+  if (write && !store->workspace) return Error(Code::kInvalidArg, "quantised rows: a write needs its workspace (null store pointer)");   // (whatever num_rows)
   if ((uintptr_t)store->codes % 4 || (uintptr_t)store->scales % 4 || (uintptr_t)store->workspace % 4)
     return Error(Code::kInvalidArg, "quantised rows: codes, scales and workspace are 4-byte aligned");
   d->codes = (uint8_t*)store->codes;

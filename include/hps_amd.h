@@ -455,7 +455,7 @@ int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dens
  *           first in the low half; 4-byte aligned (the rows' last bytes may be padding, written as zeros)
  *   scales  num_rows * hps_qrows_groups(dim, group) floats; group 0: one scale per row, else one per 16, 32, 64, 128 or 256
  *           consecutive values (the last group of a row may be shorter)
- *   workspace  hps_qrows_workspace_bytes(num_rows) bytes, zero before the first write, 4-byte aligned; a read needs none
+ *   workspace  hps_qrows_workspace_bytes(num_rows) bytes, zero before the first write, 4-byte aligned (also with 0 rows); a read needs none
  * write: per group a = max |x|, scale = fp32(a / L), L = 127 (8 bits) or 7 (4 bits), code = x / scale to the nearest integer,
  * ties to even; a < 2^-100: scale 0 and codes 0; a NaN or an infinity in the group: scale NaN, so the group reads back as NaN.
  * A slot outside [0, num_rows) is skipped; of a slot that is named several times in one call the last row stays.

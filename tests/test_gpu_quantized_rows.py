@@ -200,6 +200,9 @@ def test_nothing_to_do_and_an_empty_store():
     held = empty.write(torch.ones(3, 8, device="cuda"), slots, held=torch.zeros(3, 8, device="cuda"))
     assert torch.equal(held, torch.ones_like(held)) or (held - 1).abs().max() <= 2.0 ** -23
     assert (empty.read(slots, default_value=1.5) == 1.5).all()
+    for n in (3000, 300000):      # the ways of larger calls
+        held = empty.write(torch.ones(n, 8, device="cuda"), torch.zeros(n, dtype=torch.int64, device="cuda"), held=torch.zeros(n, 8, device="cuda"))
+        assert (held - 1).abs().max() <= 2.0 ** -23
 
 
 def test_codes_beyond_4_gib():

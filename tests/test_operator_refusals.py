@@ -47,6 +47,7 @@ def test_write_and_read_arguments():
     s = _store()
     assert _write(None) == hps.ERR_INVALID_ARG and _read(None) == hps.ERR_INVALID_ARG
     assert _write(_store(workspace=None)) == hps.ERR_INVALID_ARG
+    assert _write(_store(workspace=None, codes=None, scales=None, num_rows=0)) == hps.ERR_INVALID_ARG and "workspace" in _msg()   # (the list has a head of its own)
     assert _write(s, type=3) == hps.ERR_INVALID_ARG and "element type" in _msg()
     assert _read(s, type=-1) == hps.ERR_INVALID_ARG
     assert _write(s, rows=None) == hps.ERR_INVALID_ARG and _write(s, slots=None) == hps.ERR_INVALID_ARG
