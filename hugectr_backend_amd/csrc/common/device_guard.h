@@ -1,4 +1,5 @@
-// The calling thread's device for the length of a C entry: the entry's own device inside, the caller's again behind it.
+// The calling thread's device for the length of a C entry: the entry's own device inside, the caller's again behind it.  An error that an
+// earlier HIP call left in the thread is not this entry's (its launches ask for the last error), and the entry's own stays in its status.
 #pragma once
 #include <hip/hip_runtime_api.h>
 
@@ -13,8 +14,10 @@ class DeviceGuard {
   DeviceGuard& operator=(const DeviceGuard&) = delete;
   ~DeviceGuard() {
     if (restore_ >= 0) (void)hipSetDevice(restore_);
+    (void)hipGetLastError();
   }
   Status Enter(int device) {
+    (void)hipGetLastError();
     int now = 0;
     const bool any = hipGetDevice(&now) == hipSuccess;
     if (any && now == device) return Status::Ok();

@@ -49,6 +49,8 @@ Status LinearLayers::Create(int device, uint32_t experts, uint32_t K, uint32_t N
   if ((int)from < 0 || (int)from > 2) return Error(Code::kInvalidArg, "linear layer: unknown type of the weights ", (int)from);
   if ((int)act < 0 || (int)act > (int)Activation::kSigmoid) return Error(Code::kInvalidArg, "linear layer: unknown activation ", (int)act);
   if (!weights) return Error(Code::kInvalidArg, "linear layer: null weights");
+  if (on_device && ((uintptr_t)weights % ElemBytes(from) || (uintptr_t)bias % 4))
+    return Error(Code::kInvalidArg, "linear layer: weights and bias on the device are aligned to their elements");
   const uint32_t ksteps = (K + 31) / 32, npairs = (N + 31) / 32;
   const unsigned __int128 packed_bytes = (unsigned __int128)experts * npairs * ksteps * 2048, limit = (unsigned __int128)1 << 40;
   if (packed_bytes > limit) return Error(Code::kUnsupported, "linear layer: weights of more than 2^40 bytes");

@@ -383,3 +383,22 @@ def test_one_expert_without_offsets_takes_its_row_indexes(rows):
     got = layer.forward(x, None, rows_in=rin, rows_out=rout)
     _check(got[rout.long()], x[rin.long()], w[0], b[0], "relu")
     _check(layer.forward(x, None), x, w[0], b[0], "relu")
+
+
+def test_an_error_that_an_earlier_call_left_is_not_this_calls():
+    """A layer that does not fit the card is an error of its own call alone."""
+    import ctypes as C
+    import torch
+    from hugectr_backend_amd import hps
+    from hugectr_backend_amd.dense import LinearLayer, group_rows
+    from hugectr_backend_amd.quantized_rows import QuantizedRows
+    x, w, b = _operands(torch, 9, 64, 40, torch.float16, 1)
+    layer, store = LinearLayer(w[0], b[0]), QuantizedRows(10, 4)
+    slots = torch.arange(3, device="cuda")
+    for call in (lambda: layer.forward(x), lambda: group_rows(slots.int(), 4), lambda: store.write(torch.ones(3, 4, device="cuda"), slots),
+                 lambda: store.read(slots)):
+        h = C.c_void_p()
+        rc = hps.LIB.hps_linear_create(0, 256, 1 << 20, 512, 1, 0, 0x10000, 0, None, 0, None, C.byref(h))      # 549 GB of weights: nothing is read
+        assert rc == hps.ERR_INTERNAL and "hipMalloc" in hps.LIB.hps_last_error().decode() and not h.value
+        call()
+    _check(layer.forward(x), x, w[0], b[0], "none")

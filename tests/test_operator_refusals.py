@@ -78,7 +78,8 @@ def _create(experts=1, k=16, n=16, type=1, act=0, weights=P, wtype=0, bias=None,
 def test_layers_that_cannot_be():
     for kw, word in ((dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(k=0), "widths"), (dict(n=0), "widths"),
                      (dict(k=(1 << 20) + 1), "widths"), (dict(type=0), "fp16 or bf16"), (dict(type=7), "element type"), (dict(wtype=9), "element type"),
-                     (dict(act=5), "activation"), (dict(act=-1), "activation"), (dict(weights=None), "null weights")):
+                     (dict(act=5), "activation"), (dict(act=-1), "activation"), (dict(weights=None), "null weights"),
+                     (dict(weights=P + 2), "aligned"), (dict(weights=P + 1, wtype=1), "aligned"), (dict(bias=P + 2), "aligned")):
         assert _create(**kw) == hps.ERR_INVALID_ARG and word in _msg(), kw
     assert _create(experts=1024, k=1 << 20, n=1 << 20) == hps.ERR_UNSUPPORTED
     assert L.hps_linear_create(0, 1, 16, 16, 1, 0, P, 0, None, 1, None, None) == hps.ERR_INVALID_ARG
