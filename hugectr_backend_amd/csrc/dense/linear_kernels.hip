@@ -709,9 +709,10 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
 constexpr uint64_t kStreamBytes = 32ull << 20;
 
 // Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
-// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6; M = 2048: 64 x 64 9.1, 128 x 128 11.4; M = 8192: 64 x 64 31, 128 x
-// 128 21.6, 128 x 256 21.3; M = 65536, N = K = 256: 128 x 128 17.0, 128 x 256 15.6.  Few columns leave no room for wide tiles: M = 65536,
-// N = 64, K = 256: 64 x 64 9.2, 128 x 128 11.1.
+// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6.  A wider tile from 5/8 of the CUs on: 64 x 64 / 128 x 128 with 128 wide
+// tiles 9.6 / 12.7, 160 13.4 / 13.0, 208 17.5 / 13.6 (K = 3456: 135 39.3 / 31.6, 216 50.8 / 34.4); 128 x 128 / 128 x 256 with 112 wide tiles
+// (K = 3456) 34.4 / 46.9, 168 55.1 / 50.3; 160 (K = 1024) 19.3 / 19.3.  Few columns leave no room for wide tiles: M = 65536, N = 64, K = 256:
+// 64 x 64 9.2, 128 x 128 11.1.
 // With experts the tiles are estimated as half a tile more per expert (the grid has room for the worst case).
 template <typename T, typename OutT>
 hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, hipStream_t stream) {
@@ -719,8 +720,8 @@ hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, h
   auto tiles = [&](uint64_t bm, uint64_t bn) { return ((a.rows + bm - 1) / bm + runs / 2) * ((d.N + bn - 1) / bn); };
   if (tiles(16, 32) <= 2 * cus) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
   if (tiles(32, 32) <= 2 * cus) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
-  if (tiles(128, 128) < cus || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
-  if (tiles(128, 256) < cus || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
+  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
+  if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
   return LaunchTile<T, OutT, 128, 256, 2, 4, 3>(d, a, stream);
 }
 
