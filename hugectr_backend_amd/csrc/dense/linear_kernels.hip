@@ -713,14 +713,19 @@ constexpr uint64_t kStreamBytes = 32ull << 20;
 // tiles 9.6 / 12.7, 160 13.4 / 13.0, 208 17.5 / 13.6 (K = 3456: 135 39.3 / 31.6, 216 50.8 / 34.4); 128 x 128 / 128 x 256 with 112 wide tiles
 // (K = 3456) 34.4 / 46.9, 168 55.1 / 50.3; 160 (K = 1024) 19.3 / 19.3.  Few columns leave no room for wide tiles: M = 65536, N = 64, K = 256:
 // 64 x 64 9.2, 128 x 128 11.1.
-// With experts the tiles are estimated as half a tile more per expert (the grid has room for the worst case).
+// With experts the tiles are estimated as three quarters of one more per run, and one per run at least: past two blocks of the rows kernels a
+// CU they wait for each other (300 rows over 64 experts, 479 -> 256: rows 16 / rows 32 / 64 x 64 = 5.8 / 4.9 / 6.1; 200 rows 4.4 / 4.8 / 6.0;
+// 600 over 300, 256 -> 64: 7.4 / 7.7 / 5.5).  Runs shorter than a tile of 128 take 64 x 64: 125 rows each 10.6 us against 11.7, 250 17.5 / 15.8.
 template <typename T, typename OutT>
 hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, hipStream_t stream) {
   const uint64_t cus = (uint64_t)cu_count, runs = a.offsets ? (d.experts < a.rows ? d.experts : a.rows) : 0;
-  auto tiles = [&](uint64_t bm, uint64_t bn) { return ((a.rows + bm - 1) / bm + runs / 2) * ((d.N + bn - 1) / bn); };
+  auto tiles = [&](uint64_t bm, uint64_t bn) {
+    const uint64_t most = (a.rows + bm - 1) / bm + runs * 3 / 4;
+    return (most < runs ? runs : most) * ((d.N + bn - 1) / bn);
+  };
   if (tiles(16, 32) <= 2 * cus) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
   if (tiles(32, 32) <= 2 * cus) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
-  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
+  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64 || a.rows < runs * 128) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
   if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
   return LaunchTile<T, OutT, 128, 256, 2, 4, 3>(d, a, stream);
 }
