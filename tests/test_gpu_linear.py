@@ -402,3 +402,30 @@ def test_an_error_that_an_earlier_call_left_is_not_this_calls():
         assert rc == hps.ERR_INTERNAL and "hipMalloc" in hps.LIB.hps_last_error().decode() and not h.value
         call()
     _check(layer.forward(x), x, w[0], b[0], "none")
+
+
+@pytest.mark.parametrize("act", ["relu", "silu"])
+@pytest.mark.parametrize("m,k,n,e", [(5, 70, 40, 3), (120, 64, 64, 4), (700, 96, 128, 3), (6000, 64, 520, 5), (9000, 40, 1030, 2)])
+def test_towers_in_place_over_mul_and_residual(m, k, n, e, act):
+    """The output is its own mul, its own residual, or both; rows in order and by index; every tile size."""
+    import torch
+    from hugectr_backend_amd.dense import ExpertLayers, group_rows
+    x, w, b = _operands(torch, m, k, n, torch.float16, m, experts=e)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    ids = torch.randint(-1, e, (m,), generator=g, device="cuda").int()
+    offsets, order = group_rows(ids, e)
+    layer = ExpertLayers(w, b, activation=act)
+    off = offsets.tolist()
+    for index in (order, None):
+        for which in ("mul", "residual", "both"):
+            was = torch.randn(m, n, generator=g, device="cuda").half()
+            out = was.clone()
+            layer.forward(x, offsets, rows_in=index, rows_out=index, mul=out if which != "residual" else None,
+                          residual=out if which != "mul" else None, out=out)
+            for q in range(e):
+                rows = (order if index is not None else torch.arange(m, device="cuda"))[off[q]: off[q + 1]].long()
+                if len(rows):
+                    _check(out[rows], x[rows], w[q], b[q], act, was[rows] if which != "residual" else None, was[rows] if which != "mul" else None)
+            rest = (order if index is not None else torch.arange(m, device="cuda"))[off[e]:].long()
+            assert torch.equal(out[rest], was[rest])

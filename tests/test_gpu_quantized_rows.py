@@ -158,6 +158,31 @@ def test_a_slot_named_again_keeps_its_last_row(n, dim, R):
     assert _same(got[inside], _values(codes0, scales0, 0)[slots[inside]]) and (got[~inside] == -2.5).all()
 
 
+@pytest.mark.parametrize("dtype,bits,group", [("float16", 8, 0), ("bfloat16", 4, 32), ("float32", 4, 16)])
+@pytest.mark.parametrize("n,dim", [(900, 600), (1500, 2100), (3000, 600), (2600, 2100), (262145, 40)])
+def test_a_slot_named_again_in_every_type(n, dim, dtype, bits, group):
+    """Rows in registers and rows that are read twice, scales per group, in the three ways."""
+    import torch
+    from hugectr_backend_amd.quantized_rows import QuantizedRows
+    rng = np.random.default_rng(n + dim)
+    R = n // 3
+    rows = torch.from_numpy(_rows(rng, n, dim)).to(getattr(torch, dtype)).cuda()
+    x = rows.float().cpu().numpy()
+    slots = rng.integers(-2, R + 2, n).astype(np.int64)
+    store = QuantizedRows(R, dim, bits=bits, group=group)
+    codes, scales = _quantize(x, bits, group)
+    want_c, want_s = np.zeros((R, dim), np.int64), np.zeros((R, scales.shape[1]), np.float32)
+    last = {s: i for i, s in enumerate(slots.tolist()) if 0 <= s < R}
+    at, of = np.array(list(last)), np.array(list(last.values()))
+    want_c[at], want_s[at] = codes[of], scales[of]
+    values = torch.from_numpy(_values(codes, scales, group)).to(rows.dtype)
+    for _ in range(2):                                   # the second time over what is there
+        held = store.write(rows, torch.from_numpy(slots).cuda(), held=torch.empty_like(rows))
+        assert torch.equal(held.cpu(), values)
+        assert _same(_unpacked(store)[0], want_c) and _same(store.scales.cpu().numpy(), want_s)
+    assert not store._workspace[: store.num_rows].any()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_strided_misaligned_and_in_place_rows(dtype):
     """Rows inside a wider tensor, starting anywhere; what lies between them stays as it was; held may be the rows themselves."""
