@@ -115,6 +115,18 @@ def _link(out: Path, objs, extra=()):
           *os.environ.get("HPS_AMD_EXTRA_LDFLAGS", "").split()])
 
 
+def _torch_module(src: Path, out: Path):
+    """The operators' calls on torch tensors, a CPython module.  Its hps_* entries come from libhps_amd.so, which hps.py loads first."""
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    dirs = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", Path("/opt/rocm/include"), sysconfig.get_paths()["include"]]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{ROOT / 'include'}", *(f"-isystem{d}" for d in dirs), str(src),
+          "-o", str(out), f"-L{home / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"])
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> dict:
     jobs = jobs or min(8, os.cpu_count() or 1)
     groups = {"engine": ENGINE_SRCS, "capi": CAPI_SRCS}
@@ -149,6 +161,11 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if newer(out, deps):
             _link(out, deps, ["-ldl"])
         outs["mock_core"] = out
+    out = LIB / "hps_torch_calls.so"
+    src = CSRC / "python" / "torch_calls.cpp"
+    if force or not out.exists() or out.stat().st_mtime < max(src.stat().st_mtime, (ROOT / "include" / "hps_amd.h").stat().st_mtime):
+        _torch_module(src, out)
+    outs["torch_calls"] = out
     # native tools next to the libraries (binaries are git-ignored like the libraries; they travel with gpurun)
     tool_src = ROOT / "tools" / "triton_abi_bench.cpp"
     if tool_src.exists() and "mock" in groups:

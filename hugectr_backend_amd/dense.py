@@ -6,14 +6,11 @@ csrc/dense/; torch is used for device buffers only.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 
 import numpy as np
 
 from . import hps
-from .quantized_rows import _invalid, current_stream, elem_type, row_stride
-
-_pack_args = struct.Struct("QQQQQQiiQQQQQQQQ").pack       # an hps.LinearArgs, 0.4 us sooner than field by field
+from .quantized_rows import _invalid, calls, elem_type
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
@@ -117,66 +114,30 @@ class ExpertLayers:
                 raise _invalid(f"biases: [{w.shape[0]}, {w.shape[2]}] expected, got {tuple(b.shape)}")
         self.num_experts, self.in_dim, self.out_dim = (int(v) for v in w.shape)
         self.dtype, self.activation, self.device = dtype, activation, int(device)
-        self._index_type, self._stream = torch.int32, current_stream()
-        self._like = {t: torch.empty(0, dtype=t, device=dev) for t in (dtype, torch.float32)}   # new_empty of the same type: 0.5 us less
+        self._call, self._type = calls().linear_forward, elem_type(dtype)
         h = C.c_void_p()
         hps._check(hps.LIB.hps_linear_create(self.device, self.num_experts, self.in_dim, self.out_dim, elem_type(dtype),
                                              ACTIVATIONS[activation], w.data_ptr(), elem_type(w.dtype), b.data_ptr() if b is not None else None,
                                              1, torch.cuda.current_stream(dev).cuda_stream, C.byref(h)))
         self._h = h
 
-    def _index(self, t, n, name):
-        if t.dtype != self._index_type or t.get_device() != self.device or t.shape != (n,) or not t.is_contiguous():
-            raise _invalid(f"{name}: a contiguous vector of {n} int32 on cuda:{self.device} expected, got {t.dtype} {tuple(t.shape)} on "
-                           f"{t.device}")
-        return t.data_ptr()
-
     def forward(self, x, offsets, rows_in=None, rows_out=None, mul=None, residual=None, out=None, out_dtype=None):
         """x: CUDA `dtype` [x_rows, in_dim] (rows may be apart).  offsets: CUDA int32 [num_experts + 1]; expert e has the positions
         [offsets[e], offsets[e+1]) (clamped to the positions there are, read as their running maximum); None with one expert: all of
-        them.  rows_in / rows_out: None or
-        CUDA int32, one entry per position: the row of x it reads (outside x: zeros) and the row of out, mul and residual it has
-        (outside out: not written; a row named twice holds, element by element, the result of either).
+        them.  rows_in / rows_out: None or CUDA int32, one entry per position: the row of x it reads (outside x: zeros) and the row of
+        out, mul and residual it has (outside out: not written; a row named twice holds, element by element, the result of either).
         Without them position p is row p.  group_rows() makes offsets and such an index from expert numbers.
         out: [rows, out_dim] of `dtype` or fp32; rows of no run stay as they were.  Without `out` a new tensor of `out_dtype` is
         returned, one row per position, and rows of no run are zero (rows_out then names every row once).
         mul, residual: None or `dtype`, rows like out's; either may be `out` itself (rows_out then names no row twice).
         Runs on torch's current stream; may be captured; calls may overlap."""
-        p = rows_in if rows_in is not None else rows_out
-        rows = x.shape[0] if p is None else p.shape[0]
-        o = self._index(offsets, self.num_experts + 1, "offsets") if offsets is not None else 0
-        i = self._index(rows_in, rows, "rows_in") if rows_in is not None else 0
-        j = i if rows_out is rows_in else self._index(rows_out, rows, "rows_out") if rows_out is not None else 0
-        return self._run(x, rows, o, i, j, mul, residual, out, out_dtype)
+        return self._run(x, offsets, rows_in, rows_out, mul, residual, out, out_dtype)
 
-    def _run(self, x, rows, offsets, rows_in, rows_out, mul, residual, out, out_dtype):
-        if x.dtype != self.dtype:
-            raise _invalid(f"x: {self.dtype} expected, got {x.dtype}")
-        stride = row_stride(x, self.in_dim, "x", self.device)
-        if out is None:
-            like = self._like.get(out_dtype or self.dtype)
-            if like is None:
-                raise _invalid(f"out_dtype: {self.dtype} or torch.float32 expected, got {out_dtype}")
-            out = like.new_empty(rows, self.out_dim)
-            zero_rest, out_stride = 1, self.out_dim
-        else:
-            if out_dtype is not None and out.dtype != out_dtype:
-                raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
-            zero_rest, out_stride = 0, row_stride(out, self.out_dim, "out", self.device)
-        m, ms = (0, 0) if mul is None else self._beside(mul, out, "mul")
-        r, rs = (0, 0) if residual is None else self._beside(residual, out, "residual")
-        a = _pack_args(x.data_ptr(), stride, x.shape[0], out.data_ptr(), out_stride, out.shape[0], elem_type(out.dtype), zero_rest,
-                       m, ms, r, rs, rows, offsets, rows_in, rows_out)
-        rc = hps.LIB.hps_linear_forward(self._h, a, self._stream(self.device))
-        if rc:
-            hps._check(rc)
-        return out
-
-    def _beside(self, t, out, name):
-        stride = row_stride(t, self.out_dim, name, self.device)
-        if t.dtype != self.dtype or t.shape[0] != out.shape[0]:
-            raise _invalid(f"{name}: {out.shape[0]} rows of {self.dtype} expected, got {t.shape[0]} of {t.dtype}")
-        return t.data_ptr(), stride
+    def _run(self, x, offsets, rows_in, rows_out, mul, residual, out, out_dtype):
+        if out is not None and out_dtype is not None and out.dtype != out_dtype:
+            raise _invalid(f"out: {out_dtype} asked for, got {out.dtype}")
+        return self._call(self._h.value if self._h else 0, self.device, self._type, self.in_dim, self.out_dim, self.num_experts, x, offsets, rows_in,
+                          rows_out, mul, residual, out, self._type if out_dtype is None else elem_type(out_dtype))
 
     def close(self):
         if getattr(self, "_h", None):
@@ -202,25 +163,11 @@ class LinearLayer(ExpertLayers):
         stream; may be captured; calls may overlap."""
         if out is not None and out.shape[0] != x.shape[0]:
             raise _invalid(f"out: {x.shape[0]} rows expected, got {out.shape[0]}")
-        return self._run(x, x.shape[0], 0, 0, 0, mul, residual, out, out_dtype)
+        return self._run(x, None, None, None, mul, residual, out, out_dtype)
 
 
 def group_rows(ids, num_experts: int):
     """(offsets, order) of a stable sort of the positions by expert number: ids CUDA int32 [n]; offsets int32 [num_experts + 1],
     order int32 [n]: expert e has the positions order[offsets[e] : offsets[e+1]] in ascending order; positions whose id is outside
     [0, num_experts) come behind the last run.  num_experts <= 1024.  Runs on torch's current stream; may be captured."""
-    import torch
-    device = ids.get_device()
-    if device < 0 or ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
-        raise _invalid(f"ids: a contiguous CUDA vector of int32 expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-    if not 1 <= num_experts <= 1024:
-        raise _invalid(f"grouping: 1..1024 experts supported, got {num_experts}")
-    n = ids.shape[0]
-    offsets, order = ids.new_empty(num_experts + 1), ids.new_empty(n)
-    nbytes = int(hps.LIB.hps_group_rows_workspace_bytes(n, num_experts))
-    work = ids.new_empty((nbytes + 3) // 4) if nbytes else None
-    rc = hps.LIB.hps_group_rows_device(device, ids.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
-                                       work.data_ptr() if work is not None else None, torch._C._cuda_getCurrentRawStream(device))
-    if rc:
-        hps._check(rc)
-    return offsets, order
+    return calls().group_rows(ids, num_experts)

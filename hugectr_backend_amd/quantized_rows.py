@@ -1,6 +1,6 @@
 """Embedding rows held in 8 or 4 bits on the GPU, addressed by slot — a thin ctypes wrapper over the hps_qrows_* entry points of
 libhps_amd.so (include/hps_amd.h).  The arithmetic is the HIP code in csrc/cache/qrows_kernels.hip; torch is used for device
-buffers only.
+buffers only, its tensors are taken apart by csrc/python/torch_calls.cpp.
 """
 from __future__ import annotations
 
@@ -28,28 +28,26 @@ def elem_type(dtype) -> int:
     return t
 
 
-def current_stream():
-    """device -> hipStream_t of torch's current stream there (without the Stream object around it: 1 us of a 6-us call)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream
+_CALLS = None
 
 
-def row_stride(t, width: int, name: str, device: int) -> int:
-    """Distance of the rows of a 2-D CUDA tensor on `device` whose values lie side by side, `width` of them per row."""
-    if t.get_device() != device:
-        raise _invalid(f"{name}: a tensor on cuda:{device} expected, got one on {t.device}")
-    if t.dim() != 2 or t.shape[1] != width:
-        raise _invalid(f"{name}: rows of {width} values expected, got shape {tuple(t.shape)}")
-    rows, side = t.stride()
-    if rows == width and side == 1:
-        return width
-    if width > 1 and side != 1:
-        raise _invalid(f"{name}: the values of a row have to lie side by side")
-    if t.shape[0] <= 1:
-        return width
-    if rows < width:
-        raise _invalid(f"{name}: the rows overlap (stride {rows}, {width} values)")
-    return rows
+def calls():
+    """The native calls on torch tensors (csrc/python/torch_calls.cpp): arguments checked, outputs allocated, the C entry called."""
+    global _CALLS
+    if _CALLS is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (the module's symbols are torch's)
+        path = hps._LIBPATH.with_name("hps_torch_calls.so")
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it with `python -m hugectr_backend_amd.build`")
+        loader = importlib.machinery.ExtensionFileLoader("hps_torch_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("hps_torch_calls", loader))
+        loader.exec_module(module)
+        module.set_error(hps.HpsError)
+        _CALLS = module
+    return _CALLS
 
 
 class QuantizedRows:
@@ -79,55 +77,18 @@ class QuantizedRows:
         self._desc = hps.QRowsStore(self.codes.data_ptr(), self.scales.data_ptr(), self._workspace.data_ptr(), self.num_rows, self.dim,
                                     self.bits, self.group)
         self._desc_p = C.addressof(self._desc)
-        self._slot_type, self._stream = torch.int64, current_stream()
-        self._like = {}        # an empty tensor of every type read so far: new_empty of the same type is 0.5 us of a call less
-
-    def _slots(self, slots) -> int:
-        if slots.dtype != self._slot_type or slots.get_device() != self.device or slots.dim() != 1 or not slots.is_contiguous():
-            raise _invalid(f"slots: a contiguous vector of int64 on cuda:{self.device} expected, got {slots.dtype} {tuple(slots.shape)} "
-                           f"on {slots.device}")
-        return slots.shape[0]
+        self._write, self._read = calls().rows_write, calls().rows_read
 
     def write(self, rows, slots, held=None):
         """rows: CUDA fp32 / fp16 / bf16 [n, dim] (rows may be apart); slots: CUDA int64 [n]; a slot outside [0, num_rows) is
         skipped, of a slot named several times the last row stays.  held: None, or a tensor like `rows` (or `rows` itself) that takes
         the values the rows stand for once they are held — what read() gives from then on.  Returns `held`.  Runs on torch's
         current stream; may be captured."""
-        n = self._slots(slots)
-        stride = row_stride(rows, self.dim, "rows", self.device)
-        if rows.shape[0] != n:
-            raise _invalid(f"write: {rows.shape[0]} rows for {n} slots")
-        hp, hs = None, 0
-        if held is not None:
-            hs = row_stride(held, self.dim, "held", self.device)
-            if held.dtype != rows.dtype or held.shape[0] != n:
-                raise _invalid(f"held: {n} rows of {rows.dtype} expected, got {held.shape[0]} of {held.dtype}")
-            hp = held.data_ptr()
-        rc = hps.LIB.hps_qrows_write_device(self.device, self._desc_p, rows.data_ptr(), elem_type(rows.dtype), stride, slots.data_ptr(), n, hp,
-                                            hs, self._stream(self.device))
-        if rc:
-            hps._check(rc)
-        return held
+        return self._write(self._desc_p, self.device, self.dim, rows, slots, held)
 
     def read(self, slots, out=None, dtype=None, default_value: float = 0.0):
         """The rows at `slots` (CUDA int64 [n]) as fp32 (or `dtype`: fp16, bf16) [n, dim]; a slot outside [0, num_rows) reads as
         `default_value`.  Runs on torch's current stream; may be captured."""
-        n = self._slots(slots)
-        if out is None:
-            like = self._like.get(dtype)
-            if like is None:
-                import torch
-                elem_type(dtype or torch.float32)
-                like = self._like[dtype] = torch.empty(0, dtype=dtype or torch.float32, device=self.codes.device)
-            out, stride = like.new_empty(n, self.dim), self.dim
-        else:
-            if dtype is not None and out.dtype != dtype:
-                raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
-            stride = row_stride(out, self.dim, "out", self.device)
-            if out.shape[0] != n:
-                raise _invalid(f"out: {n} rows expected, got {out.shape[0]}")
-        rc = hps.LIB.hps_qrows_read_device(self.device, self._desc_p, slots.data_ptr(), n, default_value, out.data_ptr(),
-                                           elem_type(out.dtype), stride, self._stream(self.device))
-        if rc:
-            hps._check(rc)
-        return out
+        if out is not None and dtype is not None and out.dtype != dtype:
+            raise _invalid(f"out: {dtype} asked for, got {out.dtype}")
+        return self._read(self._desc_p, self.device, self.dim, slots, out, 0 if dtype is None else elem_type(dtype), default_value)

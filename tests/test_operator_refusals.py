@@ -178,10 +178,17 @@ def test_refusals_of_a_layer_and_of_the_wrappers():
     assert layer.forward(x[:0]).shape == (0, 6) and experts.forward(xb[:0], off).shape == (0, 6)
 
 
-def test_the_packed_arguments_are_the_struct():
-    from hugectr_backend_amd import dense
-    names = ["x", "x_stride", "x_rows", "out", "out_stride", "out_rows", "out_type", "zero_rest", "mul", "mul_stride", "residual", "residual_stride",
-             "rows", "offsets", "rows_in", "rows_out"]
-    assert names == [n for n, _ in hps.LinearArgs._fields_]
-    a = hps.LinearArgs.from_buffer_copy(dense._pack_args(*range(1, 17)))
-    assert [getattr(a, n) for n in names] == list(range(1, 17)) and C.sizeof(a) == len(dense._pack_args(*range(16)))
+def test_the_native_calls_on_torch_tensors():
+    """What the module refuses by itself, as HpsError; what is not an argument at all stays Python's own error."""
+    import torch
+    from hugectr_backend_amd.quantized_rows import calls
+    c, ids = calls(), torch.zeros(4, dtype=torch.int32)
+    for f in (lambda: c.group_rows(ids, 2), lambda: c.group_rows(3, 2), lambda: c.group_rows(ids.to_sparse(), 2), lambda: c.group_rows(ids),
+              lambda: c.rows_read(0, 0, 4, torch.zeros(3, dtype=torch.int64), None, 0, 0.0), lambda: c.rows_write(0, 0, 4, None, ids, None),
+              lambda: c.linear_forward(0, 0, 1, 4, 4, 1, ids, None, None, None, None, None, None, 1)):
+        with pytest.raises(hps.HpsError) as e:
+            f()
+        assert e.value.code == hps.ERR_INVALID_ARG and e.value.msg
+    for f in (lambda: c.group_rows(torch.zeros(4, dtype=torch.int32), "two"), lambda: c.rows_read(None, 0, 4, ids, None, 0, 0.0)):
+        with pytest.raises(TypeError):
+            f()
