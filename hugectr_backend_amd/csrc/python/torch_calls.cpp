@@ -100,7 +100,7 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int device) {
 
 void* stream_of(int device) { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream(); }
 
-// the entry, without the interpreter's lock
+// the entry alone, without the interpreter's lock: nothing that throws may be in f (addresses and streams are taken before)
 template <typename F>
 void enqueue(F&& f) {
   int rc;
@@ -136,10 +136,10 @@ PyObject* rows_write(PyObject*, PyObject* const* a, Py_ssize_t count) {
       to = held.data_ptr();
     }
     const int type = elem_type(rows.scalar_type());
-    enqueue([&] {
-      return hps_qrows_write_device(device, store, rows.data_ptr(), type, stride, (const int64_t*)slots.data_ptr(), (uint64_t)n, to, to_stride,
-                                    stream_of(device));
-    });
+    const void* from = rows.data_ptr();
+    const auto* at = (const int64_t*)slots.data_ptr();
+    void* stream = stream_of(device);
+    enqueue([&] { return hps_qrows_write_device(device, store, from, type, stride, at, (uint64_t)n, to, to_stride, stream); });
     Py_INCREF(a[5]);
     return a[5];
   });
@@ -161,10 +161,9 @@ PyObject* rows_read(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const uint64_t stride = row_stride(out, dim, "out", device);
     if (out.size(0) != n) invalid("out: ", n, " rows expected, got ", out.size(0));
     const int type = elem_type(out.scalar_type());
-    enqueue([&] {
-      return hps_qrows_read_device(device, store, (const int64_t*)slots.data_ptr(), (uint64_t)n, (float)fill, out.data_ptr(), type, stride,
-                                   stream_of(device));
-    });
+    const auto* at = (const int64_t*)slots.data_ptr();
+    void *to = out.data_ptr(), *stream = stream_of(device);
+    enqueue([&] { return hps_qrows_read_device(device, store, at, (uint64_t)n, (float)fill, to, type, stride, stream); });
     if (fresh) return THPVariable_Wrap(out);
     Py_INCREF(a[4]);
     return a[4];
@@ -212,7 +211,8 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t count) {
     };
     beside(a[10], "mul", &p.mul, &p.mul_stride);
     beside(a[11], "residual", &p.residual, &p.residual_stride);
-    enqueue([&] { return hps_linear_forward(layer, &p, stream_of(device)); });
+    void* stream = stream_of(device);
+    enqueue([&] { return hps_linear_forward(layer, &p, stream); });
     if (fresh) return THPVariable_Wrap(out);
     Py_INCREF(a[12]);
     return a[12];
@@ -234,10 +234,10 @@ PyObject* group_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const uint64_t bytes = hps_group_rows_workspace_bytes((uint64_t)n, (uint32_t)experts);
     at::Tensor work;
     if (bytes) work = empty({(int64_t)((bytes + 3) / 4)}, at::kInt, device);
-    enqueue([&] {
-      return hps_group_rows_device(device, (const int32_t*)ids.data_ptr(), (uint64_t)n, (uint32_t)experts, (int32_t*)offsets.data_ptr(),
-                                   (int32_t*)order.data_ptr(), bytes ? work.data_ptr() : nullptr, stream_of(device));
-    });
+    const auto* from = (const int32_t*)ids.data_ptr();
+    auto *starts = (int32_t*)offsets.data_ptr(), *sorted = (int32_t*)order.data_ptr();
+    void *space = bytes ? work.data_ptr() : nullptr, *stream = stream_of(device);
+    enqueue([&] { return hps_group_rows_device(device, from, (uint64_t)n, (uint32_t)experts, starts, sorted, space, stream); });
     PyObject* pair = PyTuple_New(2);
     if (!pair) throw python_error();
     PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(offsets));
