@@ -15,6 +15,7 @@ import os
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -91,7 +92,7 @@ def _deps_stamp(src: Path) -> str:
     for d in (CSRC, ROOT / "include"):
         for p in sorted(d.rglob("*.h")):
             h.update(p.read_bytes())
-    h.update(" ".join(CXXFLAGS + _flags(src)).encode())
+    h.update(" ".join(CXXFLAGS + _flags(src)).replace(str(ROOT), ".").encode())     # (a tree that was copied elsewhere is as good)
     return h.hexdigest()
 
 
@@ -161,11 +162,19 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if newer(out, deps):
             _link(out, deps, ["-ldl"])
         outs["mock_core"] = out
-    out = LIB / "hps_torch_calls.so"
-    src = CSRC / "python" / "torch_calls.cpp"
-    if force or not out.exists() or out.stat().st_mtime < max(src.stat().st_mtime, (ROOT / "include" / "hps_amd.h").stat().st_mtime):
-        _torch_module(src, out)
-    outs["torch_calls"] = out
+    try:
+        torch_version = metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        torch_version = None                       # a host that only serves through the plugin; the Python classes ask for the module
+    if torch_version:
+        out = LIB / "hps_torch_calls.so"
+        src = CSRC / "python" / "torch_calls.cpp"
+        stamp = OBJ / "python__torch_calls.stamp"
+        want = f"{_deps_stamp(src)} torch {torch_version}"      # another torch: another module
+        if force or not out.exists() or not stamp.exists() or stamp.read_text() != want:
+            _torch_module(src, out)
+            stamp.write_text(want)
+        outs["torch_calls"] = out
     # native tools next to the libraries (binaries are git-ignored like the libraries; they travel with gpurun)
     tool_src = ROOT / "tools" / "triton_abi_bench.cpp"
     if tool_src.exists() and "mock" in groups:
