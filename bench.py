@@ -31,6 +31,7 @@ import os
 import sys
 import threading
 import time
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -699,8 +700,7 @@ def main():
     class Replica:
         """One GPU's share of the deployment: its cache, its lookup sessions, its output buffers, its key batches."""
 
-    reps = []
-    for g in range(n_rep):
+    def make_replica(g):      # (a function, so that no name of it keeps a session or a cache once the replica is gone)
         rp = Replica()
         rp.g, rp.dev, rp.model, rp.cache = g, devs[g], rep_model[g], caches[g]
         with torch.cuda.device(rp.dev):
@@ -737,7 +737,9 @@ def main():
             if g > 0:
                 del rp.resident_d, rp.cdf_d
         rp.rec = []
-        reps.append(rp)
+        return rp
+
+    reps = [make_replica(g) for g in range(n_rep)]
     sessions, run, host_batches = reps[0].sessions, reps[0].run, reps[0].host_batches
     resident_d, cdf_d, resident_frac = reps[0].resident_d, reps[0].cdf_d, reps[0].resident_frac
     ncpu = effective_cpus()
@@ -766,8 +768,7 @@ def main():
     gc.disable()
     run_all(W, 0, False)
     if a.mode == "async":
-        for c in caches:
-            c.wait_async()
+        [c.wait_async() for c in caches]
     block_s = []
     thr0 = cpu_throttle_stat()
     ct0, wall0 = cpu_times(), time.perf_counter()
@@ -814,6 +815,8 @@ def main():
             for s in rp.sessions:
                 s.close()
             rp.sessions, rp.host_batches, rp.run = [], [], None
+        del rp, s
+        views = tk = tr = None
 
     # what THIS box's HBM delivers to a plain device-to-device copy (read + write bytes over time): the boxes of the pool differ by
     # up to 17 % in their HBM-bound kernels with identical code and traffic, and the line should say which kind this one is.
@@ -1332,6 +1335,7 @@ def main():
         }
     for s in sessions:
         s.close()
+    del s
 
     def guarded(name, fn):
         """A leg that can hang (kernels storing over peer mappings, RCCL groups — neither has ever run on this project's
@@ -1363,8 +1367,11 @@ def main():
     #      native load generator, then the other parameter-server tier ----
     if n_rep == 1 and not a.no_extra_legs:
         import gc
+        held = [weakref.ref(x) for x in (ps, *caches, *sessions)]
         del sessions, cache, caches, ps, made, run, host_batches, reps
+        gc.unfreeze()
         gc.collect()
+        note_what_is_left(res, held)
         torch.cuda.empty_cache()
         if not a.no_triton_leg:
             res["extra_legs"] = dict(res["extra_legs"] or {}, triton_abi=triton_abi_leg(a, hb, T, R, D, B),
@@ -1403,8 +1410,11 @@ def main():
     # the rank if the leg does not finish (a collective that hangs cannot be caught any other way).
     if n_rep > 1:
         import gc
+        held = [weakref.ref(x) for x in (ps, *caches, *sessions)]
         del sessions, cache, caches, ps, made, run, host_batches, reps
+        gc.unfreeze()
         gc.collect()
+        note_what_is_left(res, held)
         for d in sorted(set(devs)):
             with torch.cuda.device(d):
                 torch.cuda.empty_cache()
@@ -1465,6 +1475,14 @@ def silence_stdout_for_exit():
         os.close(dn)
     except Exception:  # noqa: BLE001
         pass
+
+
+def note_what_is_left(res, held):
+    """The legs behind the headline load tables as large as its own (133 GB by default): one name that still refers to its server, a
+    cache or a session, and host memory holds both."""
+    res["headline_objects_left"] = sum(r() is not None for r in held)
+    if res["headline_objects_left"]:
+        sys.stderr.write(f"[bench] {res['headline_objects_left']} objects of the headline are still referenced: its tables stay in memory\n")
 
 
 def idle_rank(a, dist, rank, world, local_rank):
