@@ -12,10 +12,12 @@ from __future__ import annotations
 import argparse
 import hashlib
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
-from importlib import metadata
+from importlib import metadata, util
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -116,14 +118,35 @@ def _link(out: Path, objs, extra=()):
           *os.environ.get("HPS_AMD_EXTRA_LDFLAGS", "").split()])
 
 
-def _torch_module(src: Path, out: Path):
-    """The operators' calls on torch tensors, a CPython module.  Its hps_* entries come from libhps_amd.so, which hps.py loads first."""
-    import sysconfig
+def _rocm_include() -> Path:
+    """The headers that belong to HIPCC."""
+    beside = Path(shutil.which(HIPCC) or HIPCC).parent.parent / "include"
+    return beside if (beside / "hip").is_dir() else Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 
+
+def _torch_home():
+    spec = util.find_spec("torch")     # (found, not imported)
+    return Path(list(spec.submodule_search_locations)[0]) if spec and spec.submodule_search_locations else None
+
+
+def torch_module_lacks(home, python_include: Path, rocm_include: Path, cxx: str):
+    """What the operators' calls on torch tensors cannot be built without here, or None.  A host that only serves through the plugin has no
+    torch, one of another kind or no Python headers; the libraries and the tools need none of it."""
+    if home is None:
+        return "torch"
+    for f in (home / "lib" / "libc10_hip.so", home / "include" / "c10" / "hip" / "HIPStream.h", python_include / "Python.h",
+              rocm_include / "hip" / "hip_runtime_api.h"):
+        if not f.exists():
+            return str(f)
+    return None if shutil.which(cxx) else cxx
+
+
+def _torch_module(src: Path, out: Path, cxx: str):
+    """The operators' calls on torch tensors, a CPython module.  Its hps_* entries come from libhps_amd.so, which hps.py loads first."""
     import torch
     home = Path(torch.__file__).resolve().parent
-    dirs = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", Path("/opt/rocm/include"), sysconfig.get_paths()["include"]]
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    dirs = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", _rocm_include(), sysconfig.get_paths()["include"]]
+    _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{ROOT / 'include'}", *(f"-isystem{d}" for d in dirs), str(src),
           "-o", str(out), f"-L{home / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"])
 
@@ -162,19 +185,6 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if newer(out, deps):
             _link(out, deps, ["-ldl"])
         outs["mock_core"] = out
-    try:
-        torch_version = metadata.version("torch")
-    except metadata.PackageNotFoundError:
-        torch_version = None                       # a host that only serves through the plugin; the Python classes ask for the module
-    if torch_version:
-        out = LIB / "hps_torch_calls.so"
-        src = CSRC / "python" / "torch_calls.cpp"
-        stamp = OBJ / "python__torch_calls.stamp"
-        want = f"{_deps_stamp(src)} torch {torch_version}"      # another torch: another module
-        if force or not out.exists() or not stamp.exists() or stamp.read_text() != want:
-            _torch_module(src, out)
-            stamp.write_text(want)
-        outs["torch_calls"] = out
     # native tools next to the libraries (binaries are git-ignored like the libraries; they travel with gpurun)
     tool_src = ROOT / "tools" / "triton_abi_bench.cpp"
     if tool_src.exists() and "mock" in groups:
@@ -185,6 +195,19 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
             _run([HIPCC, f"--offload-arch={ARCH}", "-O2", "-std=c++17", "-Wall", "-Wno-unused-result", str(tool_src), "-o", str(out),
                   "-ldl", "-pthread"])
         outs["triton_abi_bench"] = out
+    cxx = os.environ.get("CXX", "g++")
+    lacks = torch_module_lacks(_torch_home(), Path(sysconfig.get_paths()["include"]), _rocm_include(), cxx)
+    if lacks:                                       # (the Python classes of the operators say that they need the module)
+        print(f"hps_torch_calls.so left out: no {lacks}", file=sys.stderr)
+    else:
+        out = LIB / "hps_torch_calls.so"
+        src = CSRC / "python" / "torch_calls.cpp"
+        stamp = OBJ / "python__torch_calls.stamp"
+        want = f"{_deps_stamp(src)} torch {metadata.version('torch')}"      # another torch: another module
+        if force or not out.exists() or not stamp.exists() or stamp.read_text() != want:
+            _torch_module(src, out, cxx)
+            stamp.write_text(want)
+        outs["torch_calls"] = out
     if verbose:
         for k, v in outs.items():
             print(f"{k}: {v}")
