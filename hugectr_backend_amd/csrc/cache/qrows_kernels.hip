@@ -26,6 +26,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../common/launch.h"
 #include "qrows.h"
 
 namespace hps {
@@ -427,30 +428,30 @@ hipError_t WriteKept(const QRowsDesc& s, const T* rows, uint64_t row_stride, con
     return (uint32_t)((rows_of + per - 1) / per);
   };
   auto flat = [&](uint64_t each) { return (uint32_t)((n + (uint64_t)kQThreads * each - 1) / ((uint64_t)kQThreads * each)); };
+  hipError_t e;
   if (n <= kScanRows) {
-    hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kScan><<<blocks(n, 1), kQThreads, 0, stream>>>(s, rows, row_stride, slots, 0, n, held, held_stride,
-                                                                                             t.team_log, t.reduce_lanes);
-    return hipGetLastError();
+    return Launch(hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kScan>, blocks(n, 1), kQThreads, stream, s, rows, row_stride, slots, 0, n, held,
+                  held_stride, t.team_log, t.reduce_lanes);
   }
   // (in place, a row that the last kernel writes again would be read after it was replaced)
   if (n < kStampRows || (const void*)held == (const void*)rows) {
-    hps_qrows_claim_kernel<<<flat(1), kQThreads, 0, stream>>>(slots, n, s.num_rows, s.claim);
-    for (uint64_t first = 0; first < n; first += kQRowsPerLaunch) {
+    e = Launch(hps_qrows_claim_kernel, flat(1), kQThreads, stream, slots, n, s.num_rows, s.claim);
+    for (uint64_t first = 0; e == hipSuccess && first < n; first += kQRowsPerLaunch) {
       const uint64_t end = first + kQRowsPerLaunch < n ? first + kQRowsPerLaunch : n;
-      hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kClaim><<<blocks(end - first, 1), kQThreads, 0, stream>>>(
-          s, rows, row_stride, slots, first, end, held, held_stride, t.team_log, t.reduce_lanes);
+      e = Launch(hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kClaim>, blocks(end - first, 1), kQThreads, stream, s, rows, row_stride, slots, first,
+                 end, held, held_stride, t.team_log, t.reduce_lanes);
     }
-    return hipGetLastError();
+    return e;
   }
-  hps_qrows_stamp_kernel<<<flat(1), kQThreads, 0, stream>>>(slots, n, s.num_rows, s.stamp, s.listed);
-  for (uint64_t first = 0; first < n; first += kQRowsPerLaunch) {
+  e = Launch(hps_qrows_stamp_kernel, flat(1), kQThreads, stream, slots, n, s.num_rows, s.stamp, s.listed);
+  for (uint64_t first = 0; e == hipSuccess && first < n; first += kQRowsPerLaunch) {
     const uint64_t end = first + kQRowsPerLaunch < n ? first + kQRowsPerLaunch : n;
-    hps_qrows_write_kernel<T, BITS, VEC, NCH, kU, kStamp><<<blocks(end - first, kU), kQThreads, 0, stream>>>(
-        s, rows, row_stride, slots, first, end, held, held_stride, t.team_log, t.reduce_lanes);
+    e = Launch(hps_qrows_write_kernel<T, BITS, VEC, NCH, kU, kStamp>, blocks(end - first, kU), kQThreads, stream, s, rows, row_stride, slots, first,
+               end, held, held_stride, t.team_log, t.reduce_lanes);
   }
-  hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kListed><<<kListBlocks, kQThreads, 0, stream>>>(s, rows, row_stride, slots, 0, n, (T*)nullptr, 0,
-                                                                                           t.team_log, t.reduce_lanes);
-  return hipGetLastError();
+  if (e != hipSuccess) return e;
+  return Launch(hps_qrows_write_kernel<T, BITS, VEC, NCH, 1, kListed>, kListBlocks, kQThreads, stream, s, rows, row_stride, slots, 0, n, (T*)nullptr,
+                0, t.team_log, t.reduce_lanes);
 }
 
 template <typename T, int BITS, bool VEC>
@@ -471,14 +472,15 @@ hipError_t ReadTyped(const QRowsDesc& s, const int64_t* slots, uint64_t n, float
   constexpr int kU = kQWriteV<T, BITS> * sizeof(T) <= 16 ? 4 : 1;
   uint32_t group_log = 0;
   while (s.groups > 1 && (1u << group_log) < s.group) ++group_log;
-  for (uint64_t first = 0; first < n; first += kQRowsPerLaunch) {
+  hipError_t e = hipSuccess;
+  for (uint64_t first = 0; e == hipSuccess && first < n; first += kQRowsPerLaunch) {
     const uint64_t end = first + kQRowsPerLaunch < n ? first + kQRowsPerLaunch : n;
     const uint64_t per_block = (uint64_t)(kQThreads >> t.team_log) * kU;
     const uint32_t blocks = (uint32_t)((end - first + per_block - 1) / per_block);
-    hps_qrows_read_kernel<T, BITS, VEC, kU><<<blocks, kQThreads, 0, stream>>>(s, slots, first, end, default_value, (T*)out, out_stride,
-                                                                          t.team_log, group_log);
+    e = Launch(hps_qrows_read_kernel<T, BITS, VEC, kU>, blocks, kQThreads, stream, s, slots, first, end, default_value, (T*)out, out_stride, t.team_log,
+               group_log);
   }
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace

@@ -1,5 +1,6 @@
-// The calling thread's device for the length of a C entry: the entry's own device inside, the caller's again behind it.  An error that an
-// earlier HIP call left in the thread is not this entry's (its launches ask for the last error), and the entry's own stays in its status.
+// The calling thread's device for the length of a C entry: the entry's own device inside, the caller's again behind it.  The thread's last HIP
+// error stays what it was: one that the caller's earlier calls left is still there for the caller, the entry's own is in its status alone.
+// (An entry that fails while another error was pending leaves none: the runtime holds one.)
 #pragma once
 #include <hip/hip_runtime_api.h>
 
@@ -14,10 +15,9 @@ class DeviceGuard {
   DeviceGuard& operator=(const DeviceGuard&) = delete;
   ~DeviceGuard() {
     if (restore_ >= 0) (void)hipSetDevice(restore_);
-    (void)hipGetLastError();
+    if (hipPeekAtLastError() != before_) (void)hipGetLastError();
   }
   Status Enter(int device) {
-    (void)hipGetLastError();
     int now = 0;
     const bool any = hipGetDevice(&now) == hipSuccess;
     if (any && now == device) return Status::Ok();
@@ -32,6 +32,7 @@ class DeviceGuard {
   }
 
  private:
+  const hipError_t before_ = hipPeekAtLastError();
   int restore_ = -1;
 };
 

@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../common/launch.h"
 #include "linear.h"
 
 namespace hps {
@@ -208,22 +209,19 @@ hipError_t LaunchGroupRows(const int32_t* d_ids, uint64_t n, uint32_t experts, i
   uint32_t bits = 0;
   while ((experts >> bits) != 0) ++bits;   // the bins are 0 .. experts
   if (n <= kOneBlockRows) {
-    hps_group_rows_one<<<1, kGroupThreads, 0, stream>>>(d_ids, (uint32_t)n, experts, bits, d_offsets, d_order);
-    return hipGetLastError();
+    return Launch(hps_group_rows_one, 1, kGroupThreads, stream, d_ids, n, experts, bits, d_offsets, d_order);
   }
   const uint32_t tiles = (uint32_t)((n + kGroupTile - 1) / kGroupTile);
   uint32_t* counts = (uint32_t*)d_workspace;
   uint32_t* total = counts + (uint64_t)(experts + 1) * tiles;
   const uint64_t bins = experts + 1;
   const bool few = tiles <= kFewTiles && tiles * bins <= kFewCounts;
-  hps_group_rows_count<<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, few ? 1 : tiles, few ? bins : 1, counts);
-  if (few) {
-    hps_group_rows_place<false><<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
-    return hipGetLastError();
-  }
-  hps_group_rows_scan<<<experts + 1, kGroupThreads, 0, stream>>>(tiles, counts, total);
-  hps_group_rows_place<true><<<tiles, kGroupThreads, 0, stream>>>(d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
-  return hipGetLastError();
+  hipError_t e = Launch(hps_group_rows_count, tiles, kGroupThreads, stream, d_ids, n, experts, few ? 1 : tiles, few ? bins : 1, counts);
+  if (e != hipSuccess) return e;
+  if (few) return Launch(hps_group_rows_place<false>, tiles, kGroupThreads, stream, d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
+  e = Launch(hps_group_rows_scan, experts + 1, kGroupThreads, stream, tiles, counts, total);
+  if (e != hipSuccess) return e;
+  return Launch(hps_group_rows_place<true>, tiles, kGroupThreads, stream, d_ids, n, experts, bits, tiles, counts, total, d_offsets, d_order);
 }
 
 }  // namespace hps

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../common/launch.h"
 #include "linear.h"
 
 namespace hps {
@@ -730,8 +731,7 @@ hipError_t LaunchTile(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
                                                 : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, true>)
                                      : (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, true, false>
                                                 : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, false>);
-  kernel<<<(uint32_t)(m_tiles * n_tiles), 64 * WM * WN, 0, stream>>>(d, a, (uint32_t)m_tiles, (uint32_t)n_tiles);
-  return hipGetLastError();
+  return Launch(kernel, (uint32_t)(m_tiles * n_tiles), 64 * WM * WN, stream, d, a, m_tiles, n_tiles);
 }
 
 template <typename T, typename OutT, int MF, int NW>
@@ -740,8 +740,7 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
   if (m_tiles * d.npairs >= (1ull << 22)) return hipErrorInvalidConfiguration;
   const bool odd = (uintptr_t)a.x % 4 != 0 || a.x_stride % 2 != 0;
   auto* kernel = odd ? hps_linear_rows_kernel<T, OutT, MF, NW, true> : hps_linear_rows_kernel<T, OutT, MF, NW, false>;
-  kernel<<<(uint32_t)(m_tiles * d.npairs), 64 * NW, 0, stream>>>(d, a, (uint32_t)m_tiles);
-  return hipGetLastError();
+  return Launch(kernel, (uint32_t)(m_tiles * d.npairs), 64 * NW, stream, d, a, m_tiles);
 }
 
 // An output larger than the L2s together (32 MB) leaves by streaming stores: it would push out x and the weights, which the other tiles
@@ -775,9 +774,9 @@ hipError_t PackFrom(const void* w, uint32_t experts, uint32_t K, uint32_t N, voi
   const uint32_t ksteps = (K + 31) / 32, npairs = (N + 31) / 32;
   const uint64_t total = (uint64_t)experts * npairs * ksteps * 128;
   const uint32_t blocks = (uint32_t)((total + 255) / 256 < 65536 ? (total + 255) / 256 : 65536);
-  if (to == ElemType::kF16) hps_linear_pack_kernel<From, _Float16><<<blocks, 256, 0, stream>>>((const From*)w, experts, K, N, ksteps, npairs, (_Float16*)packed);
-  else hps_linear_pack_kernel<From, __bf16><<<blocks, 256, 0, stream>>>((const From*)w, experts, K, N, ksteps, npairs, (__bf16*)packed);
-  return hipGetLastError();
+  if (to == ElemType::kF16)
+    return Launch(hps_linear_pack_kernel<From, _Float16>, blocks, 256, stream, (const From*)w, experts, K, N, ksteps, npairs, (_Float16*)packed);
+  return Launch(hps_linear_pack_kernel<From, __bf16>, blocks, 256, stream, (const From*)w, experts, K, N, ksteps, npairs, (__bf16*)packed);
 }
 
 }  // namespace

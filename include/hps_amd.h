@@ -444,7 +444,8 @@ int hps_dense_forward(hps_dense_t* dense, const float* d_dense, const float* d_e
 int hps_session_lookup_interact_device(hps_session_t* session, hps_dense_t* dense, const int64_t* d_keys_flat, uint64_t batch,
                                        const float* d_dense, void* d_out_f16);
 
-/* ---- element types of the entries below */
+/* ---- element types of the entries below.  These entries leave the thread's last HIP error as it was: one that the caller's earlier calls left
+ * is neither theirs nor cleared, and their own is in the returned status alone (a call that fails while another error is pending leaves none). */
 #define HPS_TYPE_FP32 0
 #define HPS_TYPE_FP16 1
 #define HPS_TYPE_BF16 2
