@@ -941,7 +941,7 @@ int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void*
     a.offsets = args->offsets;
     a.rows_in = args->rows_in;
     a.rows_out = args->rows_out;
-    a.zero_rest = args->zero_rest != 0;
+    a.zero_rest = args->zero_rest == 2 ? kZeroUnnamed : args->zero_rest != 0 ? kZeroRest : 0;
     return layer->l->Forward(a, t, (hipStream_t)stream);
   });
 }

@@ -119,6 +119,8 @@ Status LinearLayers::Forward(const LinearArgs& a, ElemType out_type, hipStream_t
   };
   if ((a.mul && !apart(a.mul, a.mul_stride)) || (a.residual && !apart(a.residual, a.residual_stride)))
     return Error(Code::kInvalidArg, "linear forward: the output overlaps mul or residual without being the same rows of the same type");
+  if (a.zero_rest == kZeroUnnamed && a.out_rows != a.rows)
+    return Error(Code::kInvalidArg, "linear forward: rows that no position names become zeros in an output of one row per position, got ", a.out_rows, " for ", a.rows);
   DeviceGuard guard;
   HPS_RETURN_IF_ERROR(guard.Enter(device_));
   const hipError_t e = LaunchLinear(d, a, type_, out_type, cu_count_, stream);

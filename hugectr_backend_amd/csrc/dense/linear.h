@@ -17,6 +17,10 @@ enum class Activation : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmo
 constexpr uint32_t kMaxExperts = 1024;
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 
+// LinearArgs::zero_rest
+constexpr uint16_t kZeroRest = 1;      // positions of no run write zeros (else their rows stay as they were)
+constexpr uint16_t kZeroUnnamed = 2;   // and so do the rows of out that no position names (out has one row per position then)
+
 // One call's operands, all on the device.  Strides in elements.
 struct LinearArgs {
   const void* x = nullptr;            // layer type, [x_rows][x_stride]
@@ -31,7 +35,7 @@ struct LinearArgs {
   const int32_t* rows_in = nullptr;   // position -> row of x; null: the position itself
   const int32_t* rows_out = nullptr;  // position -> row of out, mul and residual; null: the position itself
   uint32_t rows = 0;                  // positions
-  uint16_t zero_rest = 0;             // positions of no run write zeros (else their rows stay as they were)
+  uint16_t zero_rest = 0;             // 0, kZeroRest, kZeroUnnamed
   uint16_t stream_out = 0;            // set by the launcher
 };
 // One kernel argument of 120 bytes or more costs the host 0.8 us a launch (2.8 -> 3.6 us, whatever its size beyond)

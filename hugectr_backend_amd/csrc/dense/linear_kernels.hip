@@ -282,6 +282,53 @@ __device__ __forceinline__ void zero_rows(const LinearDesc& d, const LinearArgs&
 }
 
 // ------------------------------------------------------------------------------------------------------------
+// Rows of out that no position names become zeros (kZeroUnnamed).  Every kernel has blocks behind its tiles for it, each with a range of
+// out's rows: it reads all of rows_out, marks what it finds of its range in LDS and zeros the rest.  No tile writes these rows, so nothing is
+// waited for, and the blocks run beside the last tiles.  Every row named, with these blocks / without:
+// 65,536 rows over 16 experts, 1024 -> 512, 91.9 / 92.4 us, 300 over 64, 479 -> 256, 7.04 / 7.00.  A launch that leaves the positions in the
+// rows they name and one that looks for them there, before the product, cost 7 us more.
+// ------------------------------------------------------------------------------------------------------------
+constexpr uint32_t kUnnamedRows = 1u << 17;   // a block's rows at most: one bit each
+
+// rows per block: a sixteenth of them, 256 at least (whole waves of rows)
+__host__ __device__ __forceinline__ uint32_t unnamed_range(uint32_t rows) {
+  const uint32_t r = ((rows + 15) / 16 + 255) / 256 * 256;
+  return r < kUnnamedRows ? r : kUnnamedRows;
+}
+__host__ __device__ __forceinline__ uint32_t unnamed_blocks(const LinearArgs& a) {
+  return a.zero_rest == kZeroUnnamed ? (a.rows + unnamed_range(a.rows) - 1) / unnamed_range(a.rows) : 0;
+}
+
+template <typename OutT, uint32_t kThreads>
+__device__ __forceinline__ void zero_unnamed(const LinearDesc& d, const LinearArgs& a, uint32_t block, uint32_t* named) {
+  const uint32_t rows = a.rows, range = unnamed_range(rows), lo = block * range, count = min(range, rows - lo);
+  for (uint32_t i = threadIdx.x; i < range / 32; i += kThreads) named[i] = 0;
+  __syncthreads();
+  auto look = [&](int32_t r) {
+    const uint32_t at = (uint32_t)r - lo;
+    if (at < count) atomicOr(&named[at / 32], 1u << (at & 31));
+  };
+  typedef u4l u4l_words __attribute__((aligned(4)));
+  const uint32_t quads = rows / 4;
+#pragma unroll 4
+  for (uint32_t q = threadIdx.x; q < quads; q += kThreads) {
+    const u4l v = reinterpret_cast<const u4l_words*>(a.rows_out)[q];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) look((int32_t)v[j]);
+  }
+  if (threadIdx.x < rows % 4) look(a.rows_out[quads * 4 + threadIdx.x]);
+  __syncthreads();
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t base = threadIdx.x - lane; base < count; base += kThreads) {   // a wave takes 64 rows
+    const uint32_t at = base + lane;
+    for (uint64_t left = __ballot(at < count && !(named[at / 32] >> (at & 31) & 1)); left; left &= left - 1) {
+      OutT* o = reinterpret_cast<OutT*>(a.out) + (uint64_t)(lo + base + (uint32_t)(__ffsll((unsigned long long)left) - 1)) * a.out_stride;
+      for (uint32_t n = lane; n < d.N; n += 64) o[n] = (OutT)0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
 // Tiles of BM rows x BN columns, WM x WN waves, K in steps of 32, NB LDS buffers.  Whole steps go from memory to LDS without passing
 // registers, NB - 1 of them on their way at once; one barrier a step.  The widest tile, 128 x 256 with three buffers, is made for two
 // workgroups on a CU: while one waits, starts or ends its tile, the other one's products run (a single 256 x 256 workgroup: 65536 x 479
@@ -323,8 +370,10 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void hps_linear_tile_kernel(Linear
   constexpr int kStage = (BM + BN) * 4;                           // 16-byte chunks of a buffer: the rows', then the weights'
   typedef typename Frag<T>::type frag;
   __shared__ __attribute__((aligned(16))) u4l lds[NB * kStage];
+  static_assert(sizeof(lds) >= kUnnamedRows / 8, "room for a block's bits");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // bands of kBand row tiles, column by column: the 64 workgroups an XCD holds at once read 8 x 8 tiles' operands, not 5 x 14
+  if (blockIdx.x >= m_tiles * n_tiles) return zero_unnamed<OutT, 64 * WM * WN>(d, a, blockIdx.x - m_tiles * n_tiles, reinterpret_cast<uint32_t*>(lds));
   const uint32_t id = xcd_order(blockIdx.x, m_tiles * n_tiles), band = id / (kBand * n_tiles), in_band = id - band * kBand * n_tiles;
   const uint32_t high_of = min(kBand, m_tiles - band * kBand), nt = in_band / high_of;
   const RowTile t = find_tile<BM>(d, a, band * kBand + in_band % high_of, lane);
@@ -633,7 +682,9 @@ __global__ __launch_bounds__(64 * NW) void hps_linear_rows_kernel(LinearDesc d, 
   constexpr int U = MF >= 4 ? 2 : 4;
   typedef typename Frag<T>::type frag;
   __shared__ __attribute__((aligned(16))) acc4 part[NW][2 * MF][64];
+  static_assert(sizeof(part) >= kUnnamedRows / 8, "room for a block's bits");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x >= m_tiles * d.npairs) return zero_unnamed<OutT, 64 * NW>(d, a, blockIdx.x - m_tiles * d.npairs, reinterpret_cast<uint32_t*>(&part[0][0][0]));
   const uint32_t id = xcd_order(blockIdx.x, m_tiles * d.npairs);
   const uint32_t pair = id / m_tiles;
   const RowTile t = find_tile<16 * MF>(d, a, id % m_tiles, lane);
@@ -731,7 +782,7 @@ hipError_t LaunchTile(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
                                                 : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, true>)
                                      : (aligned ? hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, true, false>
                                                 : hps_linear_tile_kernel<T, OutT, BM, BN, WM, WN, NB, false, false>);
-  return Launch(kernel, (uint32_t)(m_tiles * n_tiles), 64 * WM * WN, stream, d, a, m_tiles, n_tiles);
+  return Launch(kernel, (uint32_t)(m_tiles * n_tiles) + unnamed_blocks(a), 64 * WM * WN, stream, d, a, m_tiles, n_tiles);
 }
 
 template <typename T, typename OutT, int MF, int NW>
@@ -740,12 +791,16 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
   if (m_tiles * d.npairs >= (1ull << 22)) return hipErrorInvalidConfiguration;
   const bool odd = (uintptr_t)a.x % 4 != 0 || a.x_stride % 2 != 0;
   auto* kernel = odd ? hps_linear_rows_kernel<T, OutT, MF, NW, true> : hps_linear_rows_kernel<T, OutT, MF, NW, false>;
-  return Launch(kernel, (uint32_t)(m_tiles * d.npairs), 64 * NW, stream, d, a, m_tiles);
+  return Launch(kernel, (uint32_t)(m_tiles * d.npairs) + unnamed_blocks(a), 64 * NW, stream, d, a, m_tiles);
 }
 
 // An output larger than the L2s together (32 MB) leaves by streaming stores: it would push out x and the weights, which the other tiles
 // still read.  65536 x 479 -> 1024 (134 MB) 103 -> 80 us, 16384 x 1024 -> 1024 (34 MB) 33 -> 32; a smaller one may stay for its reader.
 constexpr uint64_t kStreamBytes = 32ull << 20;
+
+struct LinearTile {
+  uint32_t rows, cols;
+};
 
 // Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
 // 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6.  A wider tile from 5/8 of the CUs on: 64 x 64 / 128 x 128 with 128 wide
@@ -755,17 +810,27 @@ constexpr uint64_t kStreamBytes = 32ull << 20;
 // With experts the tiles are estimated as three quarters of one more per run, and one per run at least: past two blocks of the rows kernels a
 // CU they wait for each other (300 rows over 64 experts, 479 -> 256: rows 16 / rows 32 / 64 x 64 = 5.8 / 4.9 / 6.1; 200 rows 4.4 / 4.8 / 6.0;
 // 600 over 300, 256 -> 64: 7.4 / 7.7 / 5.5).  Runs shorter than a tile of 128 take 64 x 64: 125 rows each 10.6 us against 11.7, 250 17.5 / 15.8.
-template <typename T, typename OutT>
-hipError_t LaunchTyped(const LinearDesc& d, const LinearArgs& a, int cu_count, hipStream_t stream) {
-  const uint64_t cus = (uint64_t)cu_count, runs = a.offsets ? (d.experts < a.rows ? d.experts : a.rows) : 0;
+LinearTile TileOf(const LinearDesc& d, uint64_t rows, bool offsets, int cu_count) {
+  const uint64_t cus = (uint64_t)cu_count, runs = offsets ? (d.experts < rows ? d.experts : rows) : 0;
   auto tiles = [&](uint64_t bm, uint64_t bn) {
-    const uint64_t most = (a.rows + bm - 1) / bm + runs * 3 / 4;
+    const uint64_t most = (rows + bm - 1) / bm + runs * 3 / 4;
     return (most < runs ? runs : most) * ((d.N + bn - 1) / bn);
   };
-  if (tiles(16, 32) <= 2 * cus) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
-  if (tiles(32, 32) <= 2 * cus) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
-  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64 || a.rows < runs * 128) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
-  if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
+  if (tiles(16, 32) <= 2 * cus) return {16, 32};
+  if (tiles(32, 32) <= 2 * cus) return {32, 32};
+  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64 || rows < runs * 128) return {64, 64};
+  if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return {128, 128};
+  return {128, 256};
+}
+
+template <typename T, typename OutT>
+hipError_t LaunchTyped(const LinearDesc& d, LinearArgs a, int cu_count, hipStream_t stream) {
+  const LinearTile tile = TileOf(d, a.rows, a.offsets != nullptr, cu_count);
+  if (a.zero_rest == kZeroUnnamed && !a.rows_out) a.zero_rest = kZeroRest;   // (every row is a position's)
+  if (tile.rows == 16) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
+  if (tile.rows == 32) return LaunchRows<T, OutT, 2, 8>(d, a, stream);
+  if (tile.rows == 64) return LaunchTile<T, OutT, 64, 64, 2, 2, 4>(d, a, stream);
+  if (tile.cols == 128) return LaunchTile<T, OutT, 128, 128, 2, 4, 4>(d, a, stream);
   return LaunchTile<T, OutT, 128, 256, 2, 4, 3>(d, a, stream);
 }
 

@@ -200,7 +200,7 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t count) {
     p.out_stride = row_stride(out, out_dim, "out", device);
     p.out_rows = (uint64_t)out.size(0);
     p.out_type = elem_type(out.scalar_type());
-    p.zero_rest = fresh;
+    p.zero_rest = fresh ? 2 : 0;   // (every row of a new tensor is written, whatever rows_out names)
     auto beside = [&](PyObject* o, const char* name, const void** at, uint64_t* stride) {
       if (o == Py_None) return;
       const at::Tensor& t = tensor(o, name);

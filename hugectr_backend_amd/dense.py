@@ -128,7 +128,7 @@ class ExpertLayers:
         out, mul and residual it has (outside out: not written; a row named twice holds, element by element, the result of either).
         Without them position p is row p.  group_rows() makes offsets and such an index from expert numbers.
         out: [rows, out_dim] of `dtype` or fp32; rows of no run stay as they were.  Without `out` a new tensor of `out_dtype` is
-        returned, one row per position, and rows of no run are zero (rows_out then names every row once).
+        returned, one row per position; rows of no run, and rows that rows_out does not name, are zero.
         mul, residual: None or `dtype`, rows like out's; either may be `out` itself (rows_out then names no row twice).
         Runs on torch's current stream; may be captured; calls may overlap."""
         return self._run(x, offsets, rows_in, rows_out, mul, residual, out, out_dtype)

@@ -497,7 +497,8 @@ typedef struct hps_linear_args {
   void* out;                  /* out_type, [out_rows] rows out_stride apart; may be mul or residual itself, else apart from all inputs */
   uint64_t out_stride, out_rows;   /* (out as its own mul or residual: rows_out names no row twice) */
   int32_t out_type;           /* the layer's type or HPS_TYPE_FP32 */
-  int32_t zero_rest;          /* positions of no run: 0 = their output rows stay as they were, 1 = they become zeros */
+  int32_t zero_rest;          /* positions of no run: 0 = their output rows stay as they were, 1 = they become zeros; 2 = these and the rows of
+                                 out that no entry of rows_out names become zeros (out_rows == rows) */
   const void* mul;            /* null, or the layer's type, rows like out's */
   uint64_t mul_stride;
   const void* residual;       /* null, or the layer's type, rows like out's */
