@@ -946,6 +946,17 @@ int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void*
   });
 }
 
+int hps_linear_tile(const hps_linear_t* layer, uint64_t rows, int with_offsets, uint32_t* tile_rows, uint32_t* tile_cols) {
+  return Guard([&]() -> Status {
+    if (!layer || !tile_rows || !tile_cols) return Error(Code::kInvalidArg, "null argument");
+    if (rows == 0 || rows >= (1ull << 31)) return Error(Code::kInvalidArg, "linear tile: 1..2^31 - 1 rows expected, got ", rows);
+    const LinearTile t = layer->l->Tile(rows, with_offsets != 0);
+    *tile_rows = t.rows;
+    *tile_cols = t.cols;
+    return Status::Ok();
+  });
+}
+
 uint64_t hps_group_rows_workspace_bytes(uint64_t n, uint32_t num_experts) { return GroupRowsWorkspaceBytes(n, num_experts); }
 
 int hps_group_rows_device(int device, const int32_t* d_ids, uint64_t n, uint32_t num_experts, int32_t* d_offsets, int32_t* d_order,

@@ -55,6 +55,12 @@ hipError_t LaunchLinearPack(const void* d_w, ElemType from, uint32_t experts, ui
                             hipStream_t stream);
 hipError_t LaunchLinear(const LinearDesc& d, const LinearArgs& a, ElemType type, ElemType out_type, int cu_count, hipStream_t stream);
 
+// The rows and columns a workgroup takes: which of the five kernels a call runs
+struct LinearTile {
+  uint32_t rows, cols;
+};
+LinearTile LinearTileOf(const LinearDesc& d, uint64_t rows, bool offsets, int cu_count);
+
 uint64_t GroupRowsWorkspaceBytes(uint64_t n, uint32_t experts);
 hipError_t LaunchGroupRows(const int32_t* d_ids, uint64_t n, uint32_t experts, int32_t* d_offsets, int32_t* d_order, void* d_workspace,
                            hipStream_t stream);
@@ -68,6 +74,7 @@ class LinearLayers {
   static Status Create(int device, uint32_t experts, uint32_t K, uint32_t N, ElemType type, Activation act, const void* weights,
                        ElemType from, const float* bias, bool on_device, hipStream_t stream, LinearLayers** out);
   Status Forward(const LinearArgs& a, ElemType out_type, hipStream_t stream);
+  LinearTile Tile(uint64_t rows, bool offsets) const { return LinearTileOf(d_, rows, offsets, cu_count_); }
 
  private:
   LinearLayers() = default;

@@ -771,6 +771,27 @@ __global__ __launch_bounds__(256) void hps_linear_pack_kernel(const From* __rest
   }
 }
 
+// Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
+// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6.  A wider tile from 5/8 of the CUs on: 64 x 64 / 128 x 128 with 128 wide
+// tiles 9.6 / 12.7, 160 13.4 / 13.0, 208 17.5 / 13.6 (K = 3456: 135 39.3 / 31.6, 216 50.8 / 34.4); 128 x 128 / 128 x 256 with 112 wide tiles
+// (K = 3456) 34.4 / 46.9, 168 55.1 / 50.3; 160 (K = 1024) 19.3 / 19.3.  Few columns leave no room for wide tiles: M = 65536, N = 64, K = 256:
+// 64 x 64 9.2, 128 x 128 11.1.
+// With experts the tiles are estimated as three quarters of one more per run, and one per run at least: past two blocks of the rows kernels a
+// CU they wait for each other (300 rows over 64 experts, 479 -> 256: rows 16 / rows 32 / 64 x 64 = 5.8 / 4.9 / 6.1; 200 rows 4.4 / 4.8 / 6.0;
+// 600 over 300, 256 -> 64: 7.4 / 7.7 / 5.5).  Runs shorter than a tile of 128 take 64 x 64: 125 rows each 10.6 us against 11.7, 250 17.5 / 15.8.
+LinearTile LinearTileOf(const LinearDesc& d, uint64_t rows, bool offsets, int cu_count) {
+  const uint64_t cus = (uint64_t)cu_count, runs = offsets ? (d.experts < rows ? d.experts : rows) : 0;
+  auto tiles = [&](uint64_t bm, uint64_t bn) {
+    const uint64_t most = (rows + bm - 1) / bm + runs * 3 / 4;
+    return (most < runs ? runs : most) * ((d.N + bn - 1) / bn);
+  };
+  if (tiles(16, 32) <= 2 * cus) return {16, 32};
+  if (tiles(32, 32) <= 2 * cus) return {32, 32};
+  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64 || rows < runs * 128) return {64, 64};
+  if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return {128, 128};
+  return {128, 256};
+}
+
 namespace {
 
 template <typename T, typename OutT, int BM, int BN, int WM, int WN, int NB>
@@ -798,34 +819,9 @@ hipError_t LaunchRows(const LinearDesc& d, const LinearArgs& a, hipStream_t stre
 // still read.  65536 x 479 -> 1024 (134 MB) 103 -> 80 us, 16384 x 1024 -> 1024 (34 MB) 33 -> 32; a smaller one may stay for its reader.
 constexpr uint64_t kStreamBytes = 32ull << 20;
 
-struct LinearTile {
-  uint32_t rows, cols;
-};
-
-// Which kernel: the one whose blocks fill the card without taking too little each.  Measured with N = 1024, K = 1024 (us): M = 128: rows
-// 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6.  A wider tile from 5/8 of the CUs on: 64 x 64 / 128 x 128 with 128 wide
-// tiles 9.6 / 12.7, 160 13.4 / 13.0, 208 17.5 / 13.6 (K = 3456: 135 39.3 / 31.6, 216 50.8 / 34.4); 128 x 128 / 128 x 256 with 112 wide tiles
-// (K = 3456) 34.4 / 46.9, 168 55.1 / 50.3; 160 (K = 1024) 19.3 / 19.3.  Few columns leave no room for wide tiles: M = 65536, N = 64, K = 256:
-// 64 x 64 9.2, 128 x 128 11.1.
-// With experts the tiles are estimated as three quarters of one more per run, and one per run at least: past two blocks of the rows kernels a
-// CU they wait for each other (300 rows over 64 experts, 479 -> 256: rows 16 / rows 32 / 64 x 64 = 5.8 / 4.9 / 6.1; 200 rows 4.4 / 4.8 / 6.0;
-// 600 over 300, 256 -> 64: 7.4 / 7.7 / 5.5).  Runs shorter than a tile of 128 take 64 x 64: 125 rows each 10.6 us against 11.7, 250 17.5 / 15.8.
-LinearTile TileOf(const LinearDesc& d, uint64_t rows, bool offsets, int cu_count) {
-  const uint64_t cus = (uint64_t)cu_count, runs = offsets ? (d.experts < rows ? d.experts : rows) : 0;
-  auto tiles = [&](uint64_t bm, uint64_t bn) {
-    const uint64_t most = (rows + bm - 1) / bm + runs * 3 / 4;
-    return (most < runs ? runs : most) * ((d.N + bn - 1) / bn);
-  };
-  if (tiles(16, 32) <= 2 * cus) return {16, 32};
-  if (tiles(32, 32) <= 2 * cus) return {32, 32};
-  if (tiles(128, 128) * 8 < cus * 5 || d.N <= 64 || rows < runs * 128) return {64, 64};
-  if (tiles(128, 256) * 8 < cus * 5 || d.N <= 128) return {128, 128};
-  return {128, 256};
-}
-
 template <typename T, typename OutT>
 hipError_t LaunchTyped(const LinearDesc& d, LinearArgs a, int cu_count, hipStream_t stream) {
-  const LinearTile tile = TileOf(d, a.rows, a.offsets != nullptr, cu_count);
+  const LinearTile tile = LinearTileOf(d, a.rows, a.offsets != nullptr, cu_count);
   if (a.zero_rest == kZeroUnnamed && !a.rows_out) a.zero_rest = kZeroRest;   // (every row is a position's)
   if (tile.rows == 16) return LaunchRows<T, OutT, 1, 8>(d, a, stream);
   if (tile.rows == 32) return LaunchRows<T, OutT, 2, 8>(d, a, stream);

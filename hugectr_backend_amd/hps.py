@@ -201,6 +201,7 @@ def _load() -> C.CDLL:
         "hps_linear_create": (C.c_int, [C.c_int, u32, u32, u32, C.c_int, C.c_int, P, C.c_int, P, C.c_int, P, C.POINTER(P)]),
         "hps_linear_destroy": (None, [P]),
         "hps_linear_forward": (C.c_int, [P, P, P]),
+        "hps_linear_tile": (C.c_int, [P, u64, C.c_int, C.POINTER(u32), C.POINTER(u32)]),
         "hps_group_rows_workspace_bytes": (u64, [u64, u32]),
         "hps_group_rows_device": (C.c_int, [C.c_int, P, u64, u32, P, P, P, P]),
     }
@@ -233,7 +234,7 @@ EXPORTED_SYMBOLS = [
     "hps_shard_entry_lookup_device", "hps_shard_entry_last_stats", "hps_shard_entry_set_option", "hps_shard_entry_shard_capacity",
     "hps_shard_plan_passes", "hps_multi_gpu_selftest",
     "hps_qrows_row_bytes", "hps_qrows_groups", "hps_qrows_workspace_bytes", "hps_qrows_write_device", "hps_qrows_read_device",
-    "hps_linear_create", "hps_linear_destroy", "hps_linear_forward", "hps_group_rows_workspace_bytes", "hps_group_rows_device",
+    "hps_linear_create", "hps_linear_destroy", "hps_linear_forward", "hps_linear_tile", "hps_group_rows_workspace_bytes", "hps_group_rows_device",
 ]
 
 

@@ -517,6 +517,9 @@ int hps_linear_create(int device, uint32_t num_experts, uint32_t in_dim, uint32_
 void hps_linear_destroy(hps_linear_t* layer);
 /* Enqueued on `stream` (a hipStream_t of the layer's device), not synchronised; any number of calls at once, also captured. */
 int hps_linear_forward(hps_linear_t* layer, const hps_linear_args_t* args, void* stream);
+/* The rows and columns that a workgroup takes in a call of `rows` positions (16 x 32, 32 x 32, 64 x 64, 128 x 128 or 128 x 256): which kernel runs.
+ * For profiles and tests; results do not depend on it but for the order of the sums. */
+int hps_linear_tile(const hps_linear_t* layer, uint64_t rows, int with_offsets, uint32_t* tile_rows, uint32_t* tile_cols);
 /* The runs an expert layer needs: a stable sort of the positions 0 .. n-1 by d_ids[position].  d_offsets[num_experts + 1], d_order[n]:
  * the positions of expert e are d_order[offsets[e] .. offsets[e+1]); ids outside [0, num_experts) come behind the last run.
  * All apart from each other.  n < 2^31, num_experts <= 1024; d_workspace: hps_group_rows_workspace_bytes (may be null where that is 0), one call at a time. */
