@@ -59,6 +59,8 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) invalid(name, ": a tensor expected");
   const at::Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided) invalid(name, ": a strided tensor expected");
+  // (their memory does not hold their values)
+  if (t.is_neg() || t._is_zerotensor()) invalid(name, ": a tensor that holds its values expected, not a negated view (resolve_neg() it) or a zero tensor");
   return t;
 }
 

@@ -106,10 +106,10 @@ class ExpertLayers:
             raise _invalid(f"weights: [num_experts, in_dim, out_dim] expected, got shape {tuple(w.shape)}")
         if w.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             w = w.float()
-        w = w.to(dev).contiguous()
+        w = w.to(dev).resolve_neg().contiguous()
         b = None
         if biases is not None:
-            b = torch.as_tensor(biases).to(device=dev, dtype=torch.float32).contiguous()
+            b = torch.as_tensor(biases).to(device=dev, dtype=torch.float32).resolve_neg().contiguous()
             if tuple(b.shape) != (w.shape[0], w.shape[2]):
                 raise _invalid(f"biases: [{w.shape[0]}, {w.shape[2]}] expected, got {tuple(b.shape)}")
         self.num_experts, self.in_dim, self.out_dim = (int(v) for v in w.shape)

@@ -153,3 +153,29 @@ def test_a_new_output_by_index_in_a_replayed_graph():
             torch.cuda.synchronize()
             once = torch.bincount(names.long().clamp(max=m), minlength=m + 1)[:m]
             assert not torch.isnan(got).any() and torch.equal(got[once < 2], want[once < 2]) and (got[once == 0] == 0).all()
+
+
+def test_negated_views_are_not_read_as_what_lies_under_them():
+    """torch.imag of a conjugate is a view whose memory holds the negated values."""
+    import torch
+    from hugectr_backend_amd import hps
+    from hugectr_backend_amd.dense import ExpertLayers, LinearLayer, group_rows
+    from hugectr_backend_amd.quantized_rows import QuantizedRows
+    z = torch.complex(torch.ones(6, 1), torch.full((6, 1), 2.0)).cuda()
+    column = z.conj().imag                                       # [6, 1], stride 2
+    assert column.is_neg() and (column == -2).all()
+    store, slots = QuantizedRows(6, 1), torch.arange(6, device="cuda")
+    x = torch.ones(6, 8, dtype=torch.float16, device="cuda")
+    layer = LinearLayer(torch.eye(8))
+    neg = torch._neg_view
+    for call in (lambda: store.write(column, slots), lambda: store.write(column.resolve_neg(), slots, held=column), lambda: store.write(column.resolve_neg(), neg(slots)),
+                 lambda: store.read(slots, out=column), lambda: layer.forward(neg(x)), lambda: layer.forward(x, mul=neg(x)),
+                 lambda: layer.forward(x, residual=neg(x)), lambda: layer.forward(x, out=neg(x)), lambda: layer.forward(x, mul=torch._efficientzerotensor((6, 8), dtype=torch.float16, device="cuda")),
+                 lambda: group_rows(neg(slots.int()), 3)):
+        with pytest.raises(hps.HpsError, match="holds its values") as e:
+            call()
+        assert e.value.code == hps.ERR_INVALID_ARG
+    store.write(column.resolve_neg(), slots)
+    assert (store.read(slots) + 2).abs().max() <= 2.0 ** -22
+    w, b = neg(2 * torch.eye(8, device="cuda")), neg(torch.ones(1, 8, device="cuda"))
+    assert torch.equal(ExpertLayers(w[None], b).forward(x, torch.tensor([0, 6], dtype=torch.int32, device="cuda")), torch.full_like(x, -3))
