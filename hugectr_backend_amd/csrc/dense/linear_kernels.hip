@@ -110,11 +110,21 @@ __device__ __forceinline__ void store_words(void* p, u8l v, uint32_t left) {
   if (left & 1) __builtin_memcpy(c + 4 * (left & 6), &one, 4);
 }
 
-// erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7): one exponential and a polynomial of degree five
-__device__ __forceinline__ float erf_as(float x) {
-  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  return copysignf(fmaf(-p, __expf(-a * a), 1.f), x);
+// erfc(a / sqrt 2) / 2 for a >= 0: the Chebyshev fit of Numerical Recipes (erfcc, relative error 1.1e-7 everywhere), its argument, the exponential's
+// base and the half taken into the coefficients.  Relative, because gelu's negative tail is y * erfc(-y / sqrt 2) / 2: from an error function
+// that is good to 1.5e-7 of one the value at -5 was off by a quarter of itself.
+__device__ __forceinline__ float normal_tail(float a) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.353553391f, 1.f));
+  float p = fmaf(t, 0.246517298f, -1.18611495f);
+  p = fmaf(t, p, 2.14747446f);
+  p = fmaf(t, p, -1.63775315f);
+  p = fmaf(t, p, 0.402321582f);
+  p = fmaf(t, p, -0.26875686f);
+  p = fmaf(t, p, 0.139630057f);
+  p = fmaf(t, p, 0.539700616f);
+  p = fmaf(t, p, 1.4427292f);
+  p = fmaf(t, p, -2.82574822f);
+  return t * __builtin_amdgcn_exp2f(fmaf(a * -0.72134752f, a, p));
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -219,7 +229,10 @@ __device__ __forceinline__ acc8 activate(acc8 y, int act) {
       return y;
     case (int)Activation::kGelu:
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.5f * y[j] * (1.f + erf_as(y[j] * 0.70710678f));
+      for (int j = 0; j < 8; ++j) {
+        const float q = normal_tail(fabsf(y[j]));
+        y[j] *= y[j] < 0.f ? q : 1.f - q;
+      }
       return y;
     // (the hardware's reciprocal is good to one unit in the last place: 2^-23 of results that are rounded to 2^-11 or compared at 2^-20)
     case (int)Activation::kSilu:

@@ -230,3 +230,26 @@ def test_streamed_outputs_anywhere(m, n, k, before):
         layer.forward(x, residual=res, out=out)
         _check(torch, out, x, w, None, act, None, res)
         assert (wide[:, :before] == 3).all() and (wide[:, before + n:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("tile", list(TILES))
+def test_gelu_holds_its_relative_precision_far_out(tile, dtype):
+    """gelu(y) = y erfc(-y / sqrt 2) / 2 where it is next to nothing.  The sums are the inputs themselves (K = 1, W = 1), so what is left is the
+    activation: the fit 1.1e-7 and a dozen fp32 operations (2^-20 together), the exponential's argument y^2 / 2 + 2, rounded a few times
+    (2^-22 of it), and the output's half step."""
+    import torch
+    from hugectr_backend_amd.dense import LinearLayer
+    dt = getattr(torch, dtype)
+    m, n = TILES[tile]
+    y = torch.linspace(-12, 12, m, device="cuda").to(dt)
+    layer = LinearLayer(torch.ones(1, n), activation="gelu", dtype=dt)
+    assert _tile(layer, m) == tile
+    v = y.double()
+    want = v * torch.special.erfc(-v / math.sqrt(2)) / 2
+    for out_t in (dt, torch.float32):
+        got = layer.forward(y[:, None], out_dtype=out_t).double()
+        half = HALF[str(out_t).split(".")[1]]
+        off = want.abs() * (2.0 ** -20 + (v * v / 2 + 2) * 2.0 ** -22 + half) + (2.0 ** -25 if out_t == torch.float16 else 2.0 ** -126)
+        bad = ~((got - want[:, None]).abs() <= off[:, None])
+        assert not bad.any(), (int(bad.sum()), v[bad.any(1)][:5].tolist())

@@ -179,3 +179,21 @@ def test_negated_views_are_not_read_as_what_lies_under_them():
     assert (store.read(slots) + 2).abs().max() <= 2.0 ** -22
     w, b = neg(2 * torch.eye(8, device="cuda")), neg(torch.ones(1, 8, device="cuda"))
     assert torch.equal(ExpertLayers(w[None], b).forward(x, torch.tensor([0, 6], dtype=torch.int32, device="cuda")), torch.full_like(x, -3))
+
+
+@pytest.mark.parametrize("m", [2_200_003, 4097])
+def test_a_new_output_of_many_rows(m):
+    """More rows than sixteen blocks hold the names of; narrow rows, a name list that starts off 16 bytes."""
+    import torch
+    from hugectr_backend_amd.dense import ExpertLayers
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    x = torch.randn(m, 4, generator=g, device="cuda").half()
+    names = torch.randint(-1, m, (m + 1,), generator=g, device="cuda").int()[1:]
+    for n in (1, 3):
+        layer = ExpertLayers(torch.randn(1, 4, n, generator=g, device="cuda"), activation="sigmoid")
+        _poisoned(torch, (m, n), torch.float16)
+        got = layer.forward(x, None, rows_out=names)
+        named = torch.zeros(m + 1, dtype=torch.bool, device="cuda")
+        named[names.long() + 1] = True
+        assert not torch.isnan(got).any() and (got[~named[1:]] == 0).all() and (got[named[1:]] != 0).all()
