@@ -10,7 +10,8 @@
 //
 // The code is exact: code = rint(x / s) of the REAL quotient.  x * (1 / s) is off by at most 127 * 2^-22 = 3.1e-5, so only a product
 // within 1e-4 of a half-integer can round to the wrong side; there the sign of x - (r +- 1/2) s decides, which one fused
-// multiply-add gives exactly (rounding a nonzero number never changes its sign, and 2^-100 keeps it out of the denormals).
+// multiply-add gives exactly: rounding a nonzero number never changes its sign, and from 2^-100 on the difference is a multiple of 2^-131 at
+// least or of the value's own last place, which denormals (they are on) hold.
 //
 // A slot that is named twice in one call keeps its LAST row, whole.  Three ways, by the number of rows:
 //   few (kScan)     one launch: a block keeps its rows' slots in a table in LDS and reads the slots behind them, which leave the last

@@ -37,7 +37,7 @@ __device__ __forceinline__ uint64_t same_bin(uint32_t bin, bool live, uint32_t b
   return m;
 }
 
-// Exclusive prefix sums of value[0 .. count) for a whole block, count <= 2 * kGroupThreads; `carry` holds 2 * kGroupWaves words.
+// Exclusive prefix sums of value[0 .. count) for a whole block, count <= 2 * kGroupThreads; `carry` holds kGroupWaves words.
 // Thread t gets the sums of elements 2 t and 2 t + 1 in `a` and `b`.
 __device__ __forceinline__ void block_scan2(uint32_t va, uint32_t vb, uint32_t* carry, uint32_t& a, uint32_t& b) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

@@ -788,7 +788,8 @@ __global__ __launch_bounds__(256) void hps_linear_pack_kernel(const From* __rest
 // 16 / rows 32 / 64 x 64 = 4.0 / 5.0 / 6.3; M = 512: 8.8 / 7.4 / 6.6.  A wider tile from 5/8 of the CUs on: 64 x 64 / 128 x 128 with 128 wide
 // tiles 9.6 / 12.7, 160 13.4 / 13.0, 208 17.5 / 13.6 (K = 3456: 135 39.3 / 31.6, 216 50.8 / 34.4); 128 x 128 / 128 x 256 with 112 wide tiles
 // (K = 3456) 34.4 / 46.9, 168 55.1 / 50.3; 160 (K = 1024) 19.3 / 19.3.  Few columns leave no room for wide tiles: M = 65536, N = 64, K = 256:
-// 64 x 64 9.2, 128 x 128 11.1.
+// 64 x 64 9.2, 128 x 128 11.1.  Measured with rows on 16 bytes; rows off them go by the same rule, and some would be better off in a smaller
+// tile (4,096 x 1,024 -> 1,024, rows 1,025 apart: 128 x 128 23.6, 64 x 64 20.7).
 // With experts the tiles are estimated as three quarters of one more per run, and one per run at least: past two blocks of the rows kernels a
 // CU they wait for each other (300 rows over 64 experts, 479 -> 256: rows 16 / rows 32 / 64 x 64 = 5.8 / 4.9 / 6.1; 200 rows 4.4 / 4.8 / 6.0;
 // 600 over 300, 256 -> 64: 7.4 / 7.7 / 5.5).  Runs shorter than a tile of 128 take 64 x 64: 125 rows each 10.6 us against 11.7, 250 17.5 / 15.8.

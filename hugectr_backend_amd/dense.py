@@ -1,6 +1,6 @@
-"""Host-side handle of the dense step of BASELINE config 5 (DLRM bottom MLP + dot interaction) — a thin ctypes
+"""Host-side handle of the dense step behind a DLRM lookup (bottom MLP + dot interaction) — a thin ctypes
 wrapper over the hps_dense_* entry points of libhps_amd.so (include/hps_amd.h) — and of the layers that come behind it:
-LinearLayer, ExpertLayers (hps_linear_*) and group_rows (hps_group_rows_*).  The arithmetic is the HIP/MFMA code in
+LinearLayer, ExpertLayers (hps_linear_*) and group_rows (hps_group_rows_*), whose calls are native (csrc/python/torch_calls.cpp).  The arithmetic is the HIP/MFMA code in
 csrc/dense/; torch is used for device buffers only.
 """
 from __future__ import annotations
@@ -89,7 +89,8 @@ class ExpertLayers:
     (fp16 or bf16), sums and everything behind them in fp32, one rounding at the end.
 
     weights: [num_experts, in_dim, out_dim] (x @ W convention), biases: None or [num_experts, out_dim]; numpy arrays or torch tensors,
-    laid out for the kernels once, here.  activation: none, relu, gelu (with the error function), silu, sigmoid."""
+    laid out for the kernels once, here: a copy of them that new weights do not reach (they take a new object).  activation: none, relu,
+    gelu (with the error function), silu, sigmoid.  For serving: results carry no gradient."""
 
     def __init__(self, weights, biases=None, activation: str = "none", dtype="fp16", device: int = 0):
         import torch

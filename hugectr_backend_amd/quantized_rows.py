@@ -1,6 +1,6 @@
-"""Embedding rows held in 8 or 4 bits on the GPU, addressed by slot — a thin ctypes wrapper over the hps_qrows_* entry points of
-libhps_amd.so (include/hps_amd.h).  The arithmetic is the HIP code in csrc/cache/qrows_kernels.hip; torch is used for device
-buffers only, its tensors are taken apart by csrc/python/torch_calls.cpp.
+"""Embedding rows held in 8 or 4 bits on the GPU, addressed by slot: the hps_qrows_* entry points of libhps_amd.so (include/hps_amd.h) on
+torch tensors.  The arithmetic is the HIP code in csrc/cache/qrows_kernels.hip; write() and read() are native calls
+(csrc/python/torch_calls.cpp) that take the tensors apart and call the entry, torch holds the device buffers.
 """
 from __future__ import annotations
 
@@ -57,7 +57,8 @@ class QuantizedRows:
 
     codes   [num_rows, row_bytes] int8 (8 bits) / uint8 (4 bits, two per byte, the first in the low half); rows padded to 4 bytes
     scales  [num_rows, groups] fp32
-    Rows never written are zeros.  One write at a time per store (whatever the stream); reads beside reads are free, a read beside
+    A store of its own: which key has which slot is the caller's to keep; no session, cache or configuration of the parameter server
+    fills it or reads from it.  Rows never written are zeros.  One write at a time per store (whatever the stream); reads beside reads are free, a read beside
     a write of the same slots is the caller's to order."""
 
     def __init__(self, num_rows: int, dim: int, bits: int = 8, group: int = 0, device: int = 0):
